@@ -362,6 +362,50 @@ int rl_replay_ingest(long long num_envs, int obs_dim, int action_dim, int n_step
 int rl_reward_stats_update(long long num_envs, float gamma, const float* reward, const float* terminated,
                            const float* truncated, float* returns, float* maximum, float* running, void* stream);
 
+/* ---- token policies -------------------------------------------------------- */
+/* Operators of a policy over discrete tokens; the reference has none of them.  type: 0 fp32, 1 bf16, 3 IEEE fp16 (the
+ * product modes' numbers).  ld*: row pitches in elements.
+ *
+ * Gated feed-forward product h = act(x Wg^T) * (x Wu^T): x [rows, inputs], w [2, hidden, inputs] contiguous (gate, up),
+ * h [rows, hidden], all of `type`, fp32 accumulation; activation 0 silu, 1 gelu (erf), 2 relu.  workspace:
+ * rl_gated_workspace bytes (0 on invalid sizes), aligned to 16; two calls that may overlap need one each. */
+size_t rl_gated_workspace(int type, long long rows, int inputs, int hidden, int backward);
+int rl_gated_forward(int type, long long rows, int inputs, int hidden, int activation, const void* x, long long ldx,
+                     const void* w, void* h, long long ld_h, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients from dh: dx [rows, inputs] and dw [2, hidden, inputs] (either may be NULL; both overwritten).  Nothing
+ * is kept from the forward pass: the projections are formed again, and their gradients are rounded to `type` once.
+ * dw_fp32: dw is fp32 (else of `type`).  dx and dw must not overlap the inputs. */
+int rl_gated_backward(int type, long long rows, int inputs, int hidden, int activation, const void* x, long long ldx,
+                      const void* w, const void* dh, long long ld_dh, void* dx, long long ld_dx, void* dw, int dw_fp32,
+                      void* workspace, size_t workspace_bytes, void* stream);
+/* Distillation from a teacher's top logits.  With p = softmax(teacher_logits / T) over a row's `entries` and q =
+ * softmax(logits / T) over all classes, loss_rows = w T^2 sum_k p_k (log p_k - log q[index_k]) and dlogits = grad_scale
+ * times its gradient (dlogits NULL: loss only; it may be the logits' own buffer).  teacher_index: int32 or int64
+ * (index_bits); entries outside [0, classes) are padding, a class may be named twice.  weights [rows] NULL: 1.  A row
+ * of weight 0 or without entries has loss 0 and gradient 0.  lse (optional) receives logsumexp(logits / T).  entries
+ * up to 1024.  dlogits is of the logits' type. */
+int rl_distill_forward(const void* logits, int type, long long ld, const void* teacher_logits, int teacher_type,
+                       const void* teacher_index, int index_bits, const float* weights, long long rows, int classes,
+                       int entries, double temperature, float* loss_rows, float* lse, void* dlogits,
+                       long long ld_dlogits, float grad_scale, void* stream);
+/* The same gradient from rl_distill_forward's lse and a gradient of each row's loss. */
+int rl_distill_backward(const void* logits, int type, long long ld, const void* teacher_logits, int teacher_type,
+                        const void* teacher_index, int index_bits, const float* weights, const float* lse,
+                        const float* dloss_rows, long long rows, int classes, int entries, double temperature,
+                        void* dlogits, long long ld_dlogits, void* stream);
+/* One token a row from logits [rows, classes] (up to 2^20 classes) and uniform numbers [0, 1): weights exp(logit / T);
+ * of the classes by descending logit (equal ones by index) the first top_k (<= 0: all), of those the ones whose
+ * predecessors weigh less than top_p of them together (>= 1: all), of those the ones that weigh at least min_p times the
+ * heaviest; the first always stays.  tokens: the first kept class, by index, at which the running sum of the kept
+ * weights exceeds uniform times their sum; log_probs (optional): the log of its share of them.  T = 0: the first
+ * of the order, log_prob 0.  The *_rows arrays (optional) hold each row's setting in the scalar's place.  -infinity and
+ * NaN logits are never drawn; a row with nothing else gets token -1 and log_prob -infinity, a row whose settings
+ * (negative or infinite T, NaN) or uniform number mean nothing token -1 and NaN. */
+int rl_categorical_sample(const void* logits, int type, long long ld, long long rows, int classes, double temperature,
+                          int top_k, double top_p, double min_p, const float* temperature_rows, const int* top_k_rows,
+                          const float* top_p_rows, const float* min_p_rows, const float* uniform, long long* tokens,
+                          float* log_probs, void* stream);
+
 /* ---- PPO ------------------------------------------------------------------ */
 /* robolearn/warp/ppo.py:101-133 */
 int rl_gae(int horizon, int num_envs, float gamma, float lambda, int current_timeout_bootstrap, const float* rewards,

@@ -116,6 +116,17 @@ SIGNATURES = {
                          + [P, P]),
     "rl_reward_stats_update": (c_int, [c_ll, c_float, P, P, P, P, P, P, P]),
     "rl_actor_act": (c_int, [c_ll, c_int, c_int, c_int, c_int, P, c_ll, PP, P, P, c_float, c_float, P]),
+    # token policies
+    "rl_gated_workspace": (c_size, [c_int, c_ll, c_int, c_int, c_int]),
+    "rl_gated_forward": (c_int, [c_int, c_ll, c_int, c_int, c_int, P, c_ll, P, P, c_ll, P, c_size, P]),
+    "rl_gated_backward": (c_int, [c_int, c_ll, c_int, c_int, c_int, P, c_ll, P, P, c_ll, P, c_ll, P, c_int, P, c_size,
+                                  P]),
+    "rl_distill_forward": (c_int, [P, c_int, c_ll, P, c_int, P, c_int, P, c_ll, c_int, c_int, c_double, P, P, P, c_ll,
+                                   c_float, P]),
+    "rl_distill_backward": (c_int, [P, c_int, c_ll, P, c_int, P, c_int, P, P, P, c_ll, c_int, c_int, c_double, P, c_ll,
+                                    P]),
+    "rl_categorical_sample": (c_int, [P, c_int, c_ll, c_ll, c_int, c_double, c_int, c_double, c_double] + [P] * 7
+                              + [P]),
     # PPO
     "rl_gae": (c_int, [c_int, c_int, c_float, c_float, c_int, P, P, P, P, P, P, P, P]),
     "rl_normalize_advantages": (c_int, [P, c_ll, c_int, P, P]),

@@ -1,0 +1,305 @@
+// Distillation from a teacher's top logits: the loss of a student's row of logits and its gradient.
+//
+//   p = softmax(t / T) over the row's entries (t_k, i_k), q = softmax(z / T) over all classes,
+//   L = w T^2 sum_k p_k (log p_k - log q[i_k]),  dL/dz_j = w T (q_j - sum_{k: i_k = j} p_k).
+//
+// An entry whose index lies outside [0, classes) is padding; a row without entries (or whose entries are all -infinity)
+// and a row of weight 0 have loss 0 and gradient 0 whatever their logits hold.
+//
+// One group of threads a row, the entries in LDS.  Exponents are taken of (z - max z) / T, so that their rounding is
+// relative to the distance from the row's maximum, where the weight lies; sums are fp32 per thread and in a fixed
+// order, the few terms of the loss in 64 bits.  The gradient is written for all classes first; then, behind a barrier,
+// every entry writes its class again with all entries of that class subtracted, so that classes named twice come
+// out right and no order of writes matters.
+#include "tokens.hpp"
+
+#include <cfloat>
+#include <climits>
+#include <cmath>
+
+namespace rl {
+namespace distill {
+
+using tokens::Row;
+using tokens::Team;
+
+constexpr int kMaxEntries = 1024;
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct Params {
+    const void* logits;
+    long long ld;
+    const void* teacher;     // [rows, entries], of teacher_type
+    const void* index;       // [rows, entries], int64 or int32
+    const float* weights;    // [rows] or null
+    const float* lse_in;     // backward: logsumexp(z / T) a row
+    const float* dloss;      // backward: gradient of each row's loss
+    float* loss;             // forward: [rows]
+    float* lse_out;          // forward: [rows] or null
+    void* dlogits;           // as the logits, or null
+    long long ldd;
+    float grad_scale;        // forward: factor of the gradient
+    double temperature;
+    long long rows;
+    int classes, entries, teacher_type, index_wide;
+};
+
+__device__ __forceinline__ float teacher_value(const Params& p, long long at) {
+    if (p.teacher_type == tokens::kF32) return static_cast<const float*>(p.teacher)[at];
+    const unsigned short bits = static_cast<const unsigned short*>(p.teacher)[at];
+    return p.teacher_type == tokens::kBf16 ? tokens::Bf16::value(bits) : tokens::F16::value(bits);
+}
+
+template <typename T, int Group, int Held, bool Backward>
+__global__ __launch_bounds__(Group < 256 ? 256 : Group) void distill_kernel(Params p) {
+    typedef typename T::Store Store;
+    typedef Team<Group> G;
+    constexpr int kTeams = Group < 256 ? 256 / Group : 1;
+    constexpr int V = T::kPerChunk;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    __shared__ float scratch_all[kTeams][G::kWaves];
+    float* scratch = scratch_all[threadIdx.x / Group % kTeams];
+    // a team's entries: probability, class, and the class's logit
+    float* prob = reinterpret_cast<float*>(lds) + (threadIdx.x / Group) * 3 * p.entries;
+    int* cls = reinterpret_cast<int*>(prob + p.entries);
+    float* logit = prob + 2 * p.entries;
+
+    const long long row = blockIdx.x * static_cast<long long>(kTeams) + threadIdx.x / Group;
+    if (row >= p.rows) return;  // a team of its own wave, or none of the workgroup
+    const int t = G::thread();
+    const Store* z = static_cast<const Store*>(p.logits) + row * p.ld;
+    Store* dz = p.dlogits ? static_cast<Store*>(p.dlogits) + row * p.ldd : nullptr;
+    const float weight = p.weights ? p.weights[row] : 1.0f;
+
+    // the teacher's distribution over the row's entries
+    float top = -INFINITY;
+    bool bad = false;  // a NaN among the entries
+    for (int k = t; k < p.entries; k += Group) {
+        const long long at = row * p.entries + k;
+        const long long c = p.index_wide ? static_cast<const long long*>(p.index)[at]
+                                         : static_cast<long long>(static_cast<const int*>(p.index)[at]);
+        const bool valid = c >= 0 && c < p.classes;
+        const float x = valid ? teacher_value(p, at) : -INFINITY;
+        prob[k] = x;
+        cls[k] = valid ? static_cast<int>(c) : -1;
+        logit[k] = valid ? T::value(z[c]) : -INFINITY;
+        top = fmaxf(top, x);
+        bad |= x != x;
+    }
+    if (bad) top = INFINITY;  // infinity - infinity below: the row's loss is NaN
+    top = G::max(top, scratch);
+    const float rate = static_cast<float>(kLog2e / p.temperature);
+
+    Row<T, Group, Held> r;
+    if (weight == 0.0f || top == -INFINITY) {
+        if (!Backward && t == 0) p.loss[row] = 0.0f;
+        const bool sum_wanted = !Backward && p.lse_out;
+        if (sum_wanted) {
+            r.open(z, p.classes);
+            float m = -INFINITY;
+            r.each([&](int, const float (&v)[V], int) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) m = fmaxf(m, v[e]);
+            });
+            m = G::max(m, scratch);
+            float s = 0.0f;
+            r.each([&](int, const float (&v)[V], int) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * rate);
+            });
+            s = G::sum(s, scratch);
+            if (t == 0) p.lse_out[row] = static_cast<float>(m / p.temperature + log(static_cast<double>(s)));
+        }
+        if (dz) {
+            G::sync();
+            for (int j = t; j < p.classes; j += Group) dz[j] = Store(0);
+        }
+        return;
+    }
+
+    float mass = 0.0f;
+    for (int k = t; k < p.entries; k += Group) {
+        const float e = __builtin_amdgcn_exp2f((prob[k] - top) * rate);
+        mass += e;
+    }
+    mass = G::sum(mass, scratch);
+
+    // the student's maximum and sum
+    r.open(z, p.classes);
+    float m = -INFINITY, s = 1.0f;
+    if constexpr (!Backward) {
+        r.each([&](int, const float (&v)[V], int) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) m = fmaxf(m, v[e]);
+        });
+        m = G::max(m, scratch);
+        s = 0.0f;
+        r.each([&](int, const float (&v)[V], int) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * rate);
+        });
+        s = G::sum(s, scratch);
+    }
+
+    if constexpr (!Backward) {
+        const double log_sum = log(static_cast<double>(s)), log_mass = log(static_cast<double>(mass));
+        double terms = 0.0;
+        for (int k = t; k < p.entries; k += Group) {
+            const float e = __builtin_amdgcn_exp2f((prob[k] - top) * rate);
+            if (e == 0.0f) continue;
+            const double log_p = (static_cast<double>(prob[k]) - top) / p.temperature - log_mass;
+            const double log_q = (static_cast<double>(logit[k]) - m) / p.temperature - log_sum;
+            terms += e * (log_p - log_q);
+        }
+        // fp32 holds the sum: its terms are rounded once
+        const float total = G::sum(static_cast<float>(terms / mass), scratch);
+        if (t == 0) {
+            p.loss[row] = static_cast<float>(weight * p.temperature * p.temperature * total);
+            if (p.lse_out) p.lse_out[row] = static_cast<float>(m / p.temperature + log_sum);
+        }
+    }
+    if (!dz) return;
+
+    const float factor = static_cast<float>(weight * p.temperature * (Backward ? p.dloss[row] : p.grad_scale));
+    // q(z): forward exp2((z - m) rate) / s; backward exp(z / T - lse), with 1 / T in two pieces so that the
+    // difference is rounded once
+    const float inverse = 1.0f / s;
+    const float by = static_cast<float>(1.0 / p.temperature);
+    const float by_rest = static_cast<float>(1.0 / p.temperature - by);
+    const float lse = Backward ? p.lse_in[row] : 0.0f;
+    const auto q = [&](float x) {
+        if constexpr (Backward) {
+            x = fmaxf(x, -FLT_MAX);  // -infinity times a negative rest would be infinity
+            return __builtin_amdgcn_exp2f((__builtin_fmaf(x, by, -lse) + x * by_rest) * kLog2e);
+        } else {
+            return __builtin_amdgcn_exp2f((x - m) * rate) * inverse;
+        }
+    };
+    G::sync();  // every logit of the entries is read: the gradient may take the logits' place
+    r.each([&](int, const float (&v)[V], int first) {
+        if (first >= p.classes) return;
+        float d[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[e] = factor * q(v[e]);
+        if (first + V <= p.classes) {
+            const uint4 c = T::pack(d);
+            *reinterpret_cast<tokens::Chunk<Store>*>(dz + first) = {{c.x, c.y, c.z, c.w}};
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (first + e < p.classes) dz[first + e] = T::rounded(d[e]);
+        }
+    });
+    G::sync();  // the classes of the entries are written again below
+    for (int k = t; k < p.entries; k += Group) {
+        const int c = cls[k];
+        if (c < 0) continue;
+        float sum = 0.0f;
+        for (int o = 0; o < p.entries; ++o)
+            if (cls[o] == c) sum += __builtin_amdgcn_exp2f((prob[o] - top) * rate);
+        dz[c] = T::rounded(factor * (q(logit[k]) - sum / mass));
+    }
+}
+
+template <typename T, bool Backward>
+void launch(const Params& p, hipStream_t stream) {
+    const std::size_t lds = 3 * sizeof(float) * static_cast<std::size_t>(p.entries);
+    if (p.classes <= 64 * T::kPerChunk && p.entries <= 256) {
+        hipLaunchKernelGGL((distill_kernel<T, 64, 1, Backward>), dim3(ceil_div(p.rows, 4)), dim3(256), 4 * lds, stream, p);
+    } else {
+        hipLaunchKernelGGL((distill_kernel<T, 256, 0, Backward>), dim3(static_cast<unsigned>(p.rows)), dim3(256), lds,
+                           stream, p);
+    }
+}
+
+void run(Params& p, int type, bool backward, hipStream_t stream) {
+    if (p.rows == 0) return;
+    switch (type) {
+        case tokens::kF32:
+            backward ? launch<tokens::F32, true>(p, stream) : launch<tokens::F32, false>(p, stream);
+            break;
+        case tokens::kBf16:
+            backward ? launch<tokens::Bf16, true>(p, stream) : launch<tokens::Bf16, false>(p, stream);
+            break;
+        default:
+            backward ? launch<tokens::F16, true>(p, stream) : launch<tokens::F16, false>(p, stream);
+    }
+    check_launch("Launch distillation");
+}
+
+// The checks that both entry points share.
+Params checked(const void* logits, int type, long long ld, const void* teacher, int teacher_type, const void* index,
+               int index_bits, long long rows, int classes, int entries, double temperature, const void* dlogits,
+               long long ldd) {
+    require(tokens::known_type(type) && tokens::known_type(teacher_type),
+            "Distillation takes logits of type 0 (fp32), 1 (bf16) or 3 (fp16).");
+    require(index_bits == 32 || index_bits == 64, "Distillation takes indices of 32 or 64 bits.");
+    require(rows >= 0 && rows <= INT_MAX && classes > 0 && classes <= (1 << 24),
+            "Distillation takes 0 to 2^31 - 1 rows of 1 to 2^24 classes.");
+    require(entries > 0 && entries <= kMaxEntries, "Distillation takes 1 to 1024 teacher entries a row.");
+    require(temperature > 0.0 && std::isfinite(temperature), "The distillation temperature must be positive and finite.");
+    require(rows == 0 || (logits && teacher && index), "Distillation operands must be nonnull.");
+    require(rows <= 1 || ld >= classes, "The rows of logits overlap.");
+    require(!dlogits || rows <= 1 || ldd >= classes, "The rows of the gradient overlap.");
+    const std::size_t size = tokens::type_size(type);
+    require(aligned(logits, size) && aligned(dlogits, size) && aligned(teacher, tokens::type_size(teacher_type)) &&
+                aligned(index, index_bits / 8),
+            "Distillation operands must be aligned to their elements.");
+    if (dlogits && rows > 0) {
+        const char* a = static_cast<const char*>(logits);
+        const char* b = static_cast<const char*>(dlogits);
+        const bool apart = a + ((rows - 1) * ld + classes) * size <= b || b + ((rows - 1) * ldd + classes) * size <= a;
+        require(apart || (a == b && (rows == 1 || ld == ldd)),
+                "The gradient may take the place of the logits, or lie apart from them.");
+    }
+    Params p{};
+    p.logits = logits;
+    p.ld = ld;
+    p.teacher = teacher;
+    p.index = index;
+    p.teacher_type = teacher_type;
+    p.index_wide = index_bits == 64;
+    p.rows = rows;
+    p.classes = classes;
+    p.entries = entries;
+    p.temperature = temperature;
+    p.dlogits = const_cast<void*>(dlogits);
+    p.ldd = ldd;
+    return p;
+}
+
+}  // namespace distill
+}  // namespace rl
+
+RL_API int rl_distill_forward(const void* logits, int type, long long ld, const void* teacher_logits, int teacher_type,
+                              const void* teacher_index, int index_bits, const float* weights, long long rows,
+                              int classes, int entries, double temperature, float* loss_rows, float* lse,
+                              void* dlogits, long long ld_dlogits, float grad_scale, void* stream) {
+    return rl::guarded("rl_distill_forward", [&] {
+        rl::distill::Params p = rl::distill::checked(logits, type, ld, teacher_logits, teacher_type, teacher_index,
+                                                     index_bits, rows, classes, entries, temperature, dlogits, ld_dlogits);
+        rl::require(rows == 0 || loss_rows, "Distillation writes the rows' losses: loss_rows is null.");
+        rl::require(std::isfinite(grad_scale), "The gradient scale must be finite.");
+        p.weights = weights;
+        p.loss = loss_rows;
+        p.lse_out = lse;
+        p.grad_scale = grad_scale;
+        rl::distill::run(p, type, false, rl::as_stream(stream));
+    });
+}
+
+RL_API int rl_distill_backward(const void* logits, int type, long long ld, const void* teacher_logits, int teacher_type,
+                               const void* teacher_index, int index_bits, const float* weights, const float* lse,
+                               const float* dloss_rows, long long rows, int classes, int entries, double temperature,
+                               void* dlogits, long long ld_dlogits, void* stream) {
+    return rl::guarded("rl_distill_backward", [&] {
+        rl::distill::Params p = rl::distill::checked(logits, type, ld, teacher_logits, teacher_type, teacher_index,
+                                                     index_bits, rows, classes, entries, temperature, dlogits, ld_dlogits);
+        rl::require(rows == 0 || (lse && dloss_rows && dlogits),
+                    "The distillation gradient needs lse, the rows' loss gradients and an output.");
+        p.weights = weights;
+        p.lse_in = lse;
+        p.dloss = dloss_rows;
+        rl::distill::run(p, type, true, rl::as_stream(stream));
+    });
+}

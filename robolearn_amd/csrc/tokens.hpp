@@ -1,0 +1,211 @@
+// Rows of logits over discrete tokens: element types, and one row held by a group of threads.
+#pragma once
+
+#include "common.hpp"
+
+namespace rl {
+namespace tokens {
+
+// Element types of logits, as the product modes number them.
+enum Type : int { kF32 = 0, kBf16 = 1, kF16 = 3 };
+
+inline bool known_type(int type) { return type == kF32 || type == kBf16 || type == kF16; }
+inline int type_size(int type) { return type == kF32 ? 4 : 2; }
+
+struct F32 {
+    typedef float Store;
+    static constexpr int kPerChunk = 4;
+    static constexpr unsigned kNegInf = 0xff800000u;  // -infinity in every element of a 32-bit word
+    __device__ __forceinline__ static void unpack(const uint4& c, float (&v)[4]) {
+        v[0] = __uint_as_float(c.x), v[1] = __uint_as_float(c.y);
+        v[2] = __uint_as_float(c.z), v[3] = __uint_as_float(c.w);
+    }
+    __device__ __forceinline__ static uint4 pack(const float (&v)[4]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    __device__ __forceinline__ static float value(Store s) { return s; }
+    __device__ __forceinline__ static Store rounded(float v) { return v; }
+};
+
+struct Bf16 {
+    typedef unsigned short Store;
+    static constexpr int kPerChunk = 8;
+    static constexpr unsigned kNegInf = 0xff80ff80u;
+    __device__ __forceinline__ static void unpack(const uint4& c, float (&v)[8]) {
+        const unsigned w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ static uint4 pack(const float (&v)[8]) {
+        return make_uint4(f32x2_to_bf16x2(v[0], v[1]), f32x2_to_bf16x2(v[2], v[3]), f32x2_to_bf16x2(v[4], v[5]),
+                          f32x2_to_bf16x2(v[6], v[7]));
+    }
+    __device__ __forceinline__ static float value(Store s) { return bf16_bits_to_f32(s); }
+    __device__ __forceinline__ static Store rounded(float v) { return f32_to_bf16_bits(v); }
+};
+
+struct F16 {
+    typedef unsigned short Store;
+    static constexpr int kPerChunk = 8;
+    static constexpr unsigned kNegInf = 0xfc00fc00u;
+    __device__ __forceinline__ static void unpack(const uint4& c, float (&v)[8]) {
+        const unsigned w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f16x2_t h = __builtin_bit_cast(f16x2_t, w[i]);
+            v[2 * i] = static_cast<float>(h[0]);
+            v[2 * i + 1] = static_cast<float>(h[1]);
+        }
+    }
+    __device__ __forceinline__ static uint4 pack(const float (&v)[8]) {
+        return make_uint4(f32x2_to_f16x2(v[0], v[1]), f32x2_to_f16x2(v[2], v[3]), f32x2_to_f16x2(v[4], v[5]),
+                          f32x2_to_f16x2(v[6], v[7]));
+    }
+    __device__ __forceinline__ static float value(Store s) {
+        return static_cast<float>(__builtin_bit_cast(_Float16, s));
+    }
+    __device__ __forceinline__ static Store rounded(float v) { return f32_to_f16_bits(v); }
+};
+
+// 16 bytes at any address that suits one element: rows of odd length start anywhere.
+template <typename Store>
+struct __attribute__((packed, aligned(sizeof(Store)))) Chunk {
+    unsigned w[4];
+};
+
+// A group of Group threads (a wave, or a whole workgroup) that works on one row.
+template <int Group>
+struct Team {
+    static constexpr int kWaves = Group / kWave;
+    static_assert(Group == kWave || Group % kWave == 0, "whole waves");
+
+    __device__ __forceinline__ static int thread() { return static_cast<int>(threadIdx.x) % Group; }
+    __device__ __forceinline__ static int wave() {
+        return Group == kWave ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    }
+    // Orders the group's memory accesses (a wave's own LDS operations execute in order).
+    __device__ __forceinline__ static void sync() {
+        if constexpr (Group == kWave) {
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+        } else {
+            __syncthreads();
+        }
+    }
+    // scratch: kWaves floats of LDS; every thread receives the result
+    __device__ __forceinline__ static float sum(float v, float* scratch) {
+        v = wave_sum(v);
+        if constexpr (Group == kWave) return v;
+        __syncthreads();
+        if (threadIdx.x % kWave == 0) scratch[wave()] = v;
+        __syncthreads();
+        float total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) total += scratch[i];
+        return total;
+    }
+    __device__ __forceinline__ static float max(float v, float* scratch) {
+        v = wave_max(v);
+        if constexpr (Group == kWave) return v;
+        __syncthreads();
+        if (threadIdx.x % kWave == 0) scratch[wave()] = v;
+        __syncthreads();
+        float top = scratch[0];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, scratch[i]);
+        return top;
+    }
+};
+
+// A row of `classes` elements as 16-byte chunks: chunk t + i * Group belongs to thread t.  The last chunk may be
+// partial; chunks and elements past the row read as -infinity.  Held > 0: the row stays in the registers of the
+// group (Held chunks a thread); 0: every chunk() reads memory again.
+template <typename T, int Group, int Held>
+struct Row {
+    typedef typename T::Store Store;
+    static constexpr int V = T::kPerChunk;
+    const Store* data;
+    int full, rest;  // whole chunks, elements of the partial one
+    uint4 held[Held > 0 ? Held : 1];
+
+    __device__ __forceinline__ static uint4 nothing() {
+        return make_uint4(T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf);
+    }
+    __device__ __forceinline__ uint4 load(int c) const {
+        const Chunk<Store> x = *reinterpret_cast<const Chunk<Store>*>(data + static_cast<long long>(c) * V);
+        return make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
+    }
+    __device__ __forceinline__ uint4 load_rest() const {
+        unsigned w[4] = {T::kNegInf, T::kNegInf, T::kNegInf, T::kNegInf};
+        const Store* p = data + static_cast<long long>(full) * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (e >= rest) continue;
+            if constexpr (V == 4) {
+                w[e] = __builtin_bit_cast(unsigned, p[e]);
+            } else {
+                const unsigned bits = p[e];
+                w[e / 2] = e % 2 ? (w[e / 2] & 0xffffu) | (bits << 16) : (w[e / 2] & 0xffff0000u) | bits;
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+
+    // chunk c of the row, from memory
+    __device__ __forceinline__ uint4 read(int c) const {
+        return c < full ? load(c) : c == full && rest ? load_rest() : nothing();
+    }
+
+    // passes over the row: chunk(i) for i < passes()
+    __device__ __forceinline__ int passes() const { return (full + (rest ? 1 : 0) + Group - 1) / Group; }
+
+    __device__ __forceinline__ void open(const Store* row, int classes) {
+        data = row;
+        full = classes / V;
+        rest = classes % V;
+        if constexpr (Held > 0) {
+            const int t = Team<Group>::thread();
+#pragma unroll
+            for (int i = 0; i < Held; ++i) held[i] = t + i * Group < full ? load(t + i * Group) : nothing();
+            if (rest && t == full % Group) {
+                const uint4 last = load_rest();
+#pragma unroll
+                for (int i = 0; i < Held; ++i)
+                    if (i == full / Group) held[i] = last;
+            }
+        }
+    }
+
+    __device__ __forceinline__ uint4 chunk(int i) const {
+        if constexpr (Held > 0) return held[i];
+        else return read(Team<Group>::thread() + i * Group);
+    }
+
+    // f(i, values, index of the first value) for every pass
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        const int t = Team<Group>::thread();
+        if constexpr (Held > 0) {
+#pragma unroll
+            for (int i = 0; i < Held; ++i) {
+                float v[V];
+                T::unpack(held[i], v);
+                f(i, v, (t + i * Group) * V);
+            }
+        } else {
+            const int n = passes();
+            for (int i = 0; i < n; ++i) {
+                float v[V];
+                T::unpack(chunk(i), v);
+                f(i, v, (t + i * Group) * V);
+            }
+        }
+    }
+};
+
+}  // namespace tokens
+}  // namespace rl

@@ -410,3 +410,180 @@ def tanh_gaussian_backward(head, noise, dactions, dlog_probs, dhead, *, rows, ac
 
 def fill(x, value):
     _native.call("rl_fill", ptr(x), x.numel(), float(value), stream())
+
+
+# ---------------------------------------------------------------------------
+# Token policies
+# ---------------------------------------------------------------------------
+_TYPES = {torch.float32: FP32, torch.bfloat16: BF16, torch.float16: FP16}
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
+
+
+def _type(tensor, name):
+    code = _TYPES.get(tensor.dtype)
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {tensor.dtype}.")
+    return code
+
+
+def _current(*tensors):
+    """All on the current device, on whose current stream the call is enqueued."""
+    device = None
+    for tensor in tensors:
+        if tensor is None:
+            continue
+        if not tensor.is_cuda:
+            raise ValueError(f"Every tensor must be on the GPU, got one on {tensor.device}.")
+        if device is None:
+            device = torch.cuda.current_device()
+        if tensor.get_device() != device:
+            raise ValueError(f"Every tensor must be on the current GPU (cuda:{device}), got one on {tensor.device}.")
+
+
+def _matrix(tensor, shape, name, dtype=None):
+    """Row pitch of a [rows, columns] tensor whose rows are contiguous and do not overlap."""
+    if dtype is not None and tensor.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {tensor.dtype}.")
+    if tuple(tensor.shape) != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(tensor.shape)}.")
+    rows, columns = shape
+    pitch, step = tensor.stride()
+    if rows <= 1:
+        pitch = max(pitch, columns)
+    if (columns > 1 and step != 1) or pitch < columns:
+        raise ValueError(f"{name} needs contiguous rows that do not overlap.")
+    return pitch
+
+
+def _vector(tensor, rows, name, dtype=torch.float32):
+    if tensor.dtype != dtype or tuple(tensor.shape) != (rows,) or not tensor.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {rows} values, got "
+                         f"{tensor.dtype} {list(tensor.shape)}.")
+
+
+def gated_workspace(rows, inputs, hidden, dtype, backward=False) -> int:
+    """Bytes of workspace that gated_forward (backward: gated_backward) needs."""
+    if dtype not in _TYPES:
+        raise ValueError(f"Gated products take float32, bfloat16 or float16, got {dtype}.")
+    size = _native.load().rl_gated_workspace(_TYPES[dtype], rows, inputs, hidden, int(backward))
+    if size == 0 and _native.last_error():
+        raise ValueError(_native.last_error())
+    return size
+
+
+def _gated_operands(x, w, activation):
+    code = _type(x, "x")
+    if x.dim() != 2 or w.dim() != 3 or w.shape[0] != 2 or w.shape[2] != x.shape[1]:
+        raise ValueError(f"Gated products take x [rows, inputs] and w [2, hidden, inputs], got {list(x.shape)} and "
+                         f"{list(w.shape)}.")
+    if w.dtype != x.dtype or not w.is_contiguous():
+        raise ValueError(f"w must be contiguous and {x.dtype}, got {w.dtype}.")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(_ACTIVATIONS)}, got {activation!r}.")
+    return code, x.shape[0], x.shape[1], w.shape[1], _matrix(x, tuple(x.shape), "x")
+
+
+def gated_forward(x, w, h, *, activation="silu", workspace=None):
+    """h = act(x w[0]^T) * (x w[1]^T) in one launch (fp32: a product and a pass): x [rows, inputs], w [2, hidden,
+    inputs], h [rows, hidden], one type; x and h may have row pitches.  workspace: gated_workspace bytes; calls that
+    may overlap (other streams, other graphs) need one each."""
+    code, rows, inputs, hidden, ldx = _gated_operands(x, w, activation)
+    ld_h = _matrix(h, (rows, hidden), "h", x.dtype)
+    _current(x, w, h, workspace)
+    _native.call("rl_gated_forward", code, rows, inputs, hidden, _ACTIVATIONS[activation], x.data_ptr(), ldx,
+                 w.data_ptr(), h.data_ptr(), ld_h, ptr(workspace),
+                 0 if workspace is None else workspace.numel() * workspace.element_size(), stream())
+
+
+def gated_backward(x, w, dh, dx, dw, *, activation="silu", workspace=None):
+    """Gradients of gated_forward from dh: dx (x's shape) and dw (w's shape; x's type or float32), both overwritten,
+    either None.  The projections are formed again from x and w."""
+    code, rows, inputs, hidden, ldx = _gated_operands(x, w, activation)
+    ld_dh = _matrix(dh, (rows, hidden), "dh", x.dtype)
+    ld_dx = 0 if dx is None else _matrix(dx, (rows, inputs), "dx", x.dtype)
+    if dw is not None and (dw.shape != w.shape or not dw.is_contiguous() or dw.dtype not in (x.dtype, torch.float32)):
+        raise ValueError(f"dw must be contiguous, {list(w.shape)} and {x.dtype} or float32, got {list(dw.shape)} "
+                         f"{dw.dtype}.")
+    _current(x, w, dh, dx, dw, workspace)
+    _native.call("rl_gated_backward", code, rows, inputs, hidden, _ACTIVATIONS[activation], x.data_ptr(), ldx,
+                 w.data_ptr(), dh.data_ptr(), ld_dh, ptr(dx), ld_dx, ptr(dw),
+                 int(dw is not None and dw.dtype == torch.float32), ptr(workspace),
+                 0 if workspace is None else workspace.numel() * workspace.element_size(), stream())
+
+
+def _distill_operands(logits, teacher_logits, teacher_index, weights, temperature):
+    code = _type(logits, "logits")
+    if logits.dim() != 2 or teacher_logits.dim() != 2 or teacher_logits.shape[0] != logits.shape[0]:
+        raise ValueError(f"Distillation takes logits [rows, classes] and teacher logits [rows, entries], got "
+                         f"{list(logits.shape)} and {list(teacher_logits.shape)}.")
+    rows, classes = logits.shape
+    if teacher_index.shape != teacher_logits.shape or teacher_index.dtype not in (torch.int32, torch.int64):
+        raise ValueError("The teacher's index must be int32 or int64, one for each of its logits.")
+    if not teacher_logits.is_contiguous() or not teacher_index.is_contiguous():
+        raise ValueError("The teacher's logits and index must be contiguous.")
+    if not temperature > 0:
+        raise ValueError(f"temperature must be positive, got {temperature}.")
+    if weights is not None:
+        _vector(weights, rows, "weights")
+    return (code, _matrix(logits, (rows, classes), "logits"), rows, classes, teacher_logits.shape[1],
+            _type(teacher_logits, "teacher_logits"), 32 if teacher_index.dtype == torch.int32 else 64)
+
+
+def distill_forward(logits, teacher_logits, teacher_index, loss_rows, *, temperature=1.0, weights=None, lse=None,
+                    dlogits=None, grad_scale=1.0):
+    """loss_rows[n] = weight T^2 KL(teacher || student) of row n at temperature T, the teacher's distribution over its
+    `entries` top logits (indices outside [0, classes) are padding); dlogits (the logits' type, their own buffer or
+    another) receives grad_scale times the gradient, lse logsumexp(logits / T) for distill_backward."""
+    code, ld, rows, classes, entries, teacher, bits = _distill_operands(logits, teacher_logits, teacher_index, weights,
+                                                                        temperature)
+    _vector(loss_rows, rows, "loss_rows")
+    if lse is not None:
+        _vector(lse, rows, "lse")
+    ldd = 0 if dlogits is None else _matrix(dlogits, (rows, classes), "dlogits", logits.dtype)
+    _current(logits, teacher_logits, teacher_index, weights, loss_rows, lse, dlogits)
+    _native.call("rl_distill_forward", logits.data_ptr(), code, ld, teacher_logits.data_ptr(), teacher,
+                 teacher_index.data_ptr(), bits, ptr(weights), rows, classes, entries, float(temperature),
+                 loss_rows.data_ptr(), ptr(lse), ptr(dlogits), ldd, float(grad_scale), stream())
+
+
+def distill_backward(logits, teacher_logits, teacher_index, lse, dloss_rows, dlogits, *, temperature=1.0, weights=None):
+    """dlogits = dloss_rows[n] times the gradient of distill_forward's loss_rows[n], from its lse; dlogits may be the
+    logits' own buffer."""
+    code, ld, rows, classes, entries, teacher, bits = _distill_operands(logits, teacher_logits, teacher_index, weights,
+                                                                        temperature)
+    _vector(lse, rows, "lse")
+    _vector(dloss_rows, rows, "dloss_rows")
+    ldd = _matrix(dlogits, (rows, classes), "dlogits", logits.dtype)
+    _current(logits, teacher_logits, teacher_index, weights, lse, dloss_rows, dlogits)
+    _native.call("rl_distill_backward", logits.data_ptr(), code, ld, teacher_logits.data_ptr(), teacher,
+                 teacher_index.data_ptr(), bits, ptr(weights), lse.data_ptr(), dloss_rows.data_ptr(), rows, classes,
+                 entries, float(temperature), dlogits.data_ptr(), ldd, stream())
+
+
+def categorical_sample(logits, uniform, tokens, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, log_probs=None):
+    """tokens[n] (int64) drawn from softmax(logits[n] / temperature) after top-k, top-p and min-p, by uniform[n] of
+    [0, 1); log_probs receives the token's log-probability among what the filters kept.  Each setting is a number or a
+    tensor of one per row (float32; top_k int32).  Masked logits are -inf or NaN; a row without any other, or with a
+    setting that means nothing, gets token -1."""
+    code = _type(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError(f"Sampling takes logits [rows, classes], got {list(logits.shape)}.")
+    rows, classes = logits.shape
+    ld = _matrix(logits, (rows, classes), "logits")
+    _vector(uniform, rows, "uniform")
+    _vector(tokens, rows, "tokens", torch.int64)
+    if log_probs is not None:
+        _vector(log_probs, rows, "log_probs")
+    scalars, arrays = [], []
+    for name, value, none, dtype in (("temperature", temperature, 1.0, torch.float32), ("top_k", top_k, 0, torch.int32),
+                                     ("top_p", top_p, 1.0, torch.float32), ("min_p", min_p, 0.0, torch.float32)):
+        if isinstance(value, torch.Tensor):
+            _vector(value, rows, name, dtype)
+            scalars.append(none)
+            arrays.append(value)
+        else:
+            scalars.append(value)
+            arrays.append(None)
+    _current(logits, uniform, tokens, log_probs, *arrays)
+    _native.call("rl_categorical_sample", logits.data_ptr(), code, ld, rows, classes, *scalars, *map(ptr, arrays),
+                 uniform.data_ptr(), tokens.data_ptr(), ptr(log_probs), stream())
