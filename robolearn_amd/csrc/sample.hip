@@ -10,16 +10,16 @@
 // first of the order.
 //
 // Which token is drawn is a comparison of a long sum with a border, so weights are 64-bit fixed point: exp in fp64,
-// rounded once to a multiple of 2^-43 (2^-44 off at most; 2^20 classes of weight 1 sum to 2^63).  Integer sums have no
-// order: histograms by LDS atomics and sums over waves in any order give the same token on every run.
+// rounded once to a multiple of 2^-43 (2^20 classes of weight 1 sum to 2^63).  Integer sums have no order: histograms by
+// LDS atomics and sums over waves in any order give the same token on every run.
 //
-// One group of threads a row.  No sort: a cut (top-k by counts, top-p by mass) is found from a histogram over the
-// distance to the maximum, 1024 bins of which the border lies in one, and then by digits of the order-preserving bits
-// of the logits in that bin.  The result is a border key, how many tokens of exactly that key stay (by index), and the
-// mass above.  The last pass sums the kept weights of 64-chunk segments in index order; the segment that holds the
-// token is scanned by one wave.
+// No row is sorted.  A cut of the order (top-k by counts, top-p by mass) is a border key (the order-preserving bits of
+// the logits) and how many tokens of exactly that key stay, by index.  Rows of up to 1024 classes: one wave a row, E
+// consecutive classes a lane, the border by bisection of the key's bits.  Longer rows: one workgroup a row, in registers
+// where they fit, with the paths below.
 #include "tokens.hpp"
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -32,11 +32,7 @@ using tokens::Team;
 typedef unsigned long long u64;
 
 constexpr int kMaxClasses = 1 << 20;
-constexpr int kBins = 1024;
-constexpr int kBinsPerLane = kBins / kWave;
-constexpr int kDigit = 10;             // bits of a digit: a bin each
-static_assert(kBins == 1 << kDigit, "a bin for each digit");
-constexpr float kBinsPerUnit = 32.0f;  // linear bins of 1/32 of (max - z) / T: 32 units until the last one
+constexpr double kScale = 0x1p43;  // weight 1
 
 struct Params {
     const void* logits;
@@ -51,53 +47,292 @@ struct Params {
     float* log_probs;
 };
 
+// One row's settings.
+struct Settings {
+    double temperature, per_t, top_p;
+    u64 min_weight;  // fixed point
+    int top_k;
+    float u;
+    bool valid;
+
+    __device__ __forceinline__ Settings(const Params& p, long long r) {
+        temperature = p.temperatures ? p.temperatures[r] : p.temperature;
+        top_p = p.top_ps ? p.top_ps[r] : p.top_p;
+        const double min_p = p.min_ps ? p.min_ps[r] : p.min_p;
+        top_k = p.top_ks ? p.top_ks[r] : p.top_k;
+        u = p.uniform[r];
+        valid = temperature >= 0.0 && temperature < INFINITY && top_p == top_p && min_p == min_p && u == u;
+        per_t = temperature > 0.0 ? 1.0 / temperature : 0.0;
+        min_weight = static_cast<u64>(ceil(fmax(fmin(min_p, 1.0), 0.0) * kScale));
+    }
+    // only the first of the order can stay
+    __device__ __forceinline__ bool one() const { return temperature == 0.0 || top_p <= 0.0 || top_k == 1; }
+    __device__ __forceinline__ double target(u64 total) const {
+        return fmax(fmin(static_cast<double>(u), 1.0 - 0x1p-50), 0.0) * static_cast<double>(total);
+    }
+};
+
 // Bits that order as the values do (NaN excluded, -0 as 0).
 __device__ __forceinline__ unsigned ordered(float z) {
     const unsigned b = __float_as_uint(z + 0.0f);
     return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
-
+// The logit whose ordered bits are `key`.
+__device__ __forceinline__ float from_ordered(unsigned key) {
+    return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+}
 __device__ __forceinline__ bool masked(float z) { return !(z > -INFINITY); }  // -infinity or NaN
 
-// exp((z - m) / T) in 64 bits; m itself weighs 1 whatever it is.
-__device__ __forceinline__ double weight(float z, float m, double per_t) {
-    if (z == m) return 1.0;
-    if (masked(z)) return 0.0;
-    return exp((static_cast<double>(z) - static_cast<double>(m)) * per_t);
+// exp((z - m) / T) as a multiple of 2^-43.  With t = (z - m) 32 log2(e) / T = 32 e + i + f, |f| <= 1/2, it is 2^e times
+// 2^(i / 32), from a table of 32 (one LDS bank pair each), times the Taylor sum of exp(f ln2 / 32) to the fifth order, which
+// leaves (ln2 / 64)^6 / 720 = 2e-15 of it.  17 instructions against about 45 of exp().
+constexpr int kTable = 32;
+__device__ __forceinline__ void fill_table(double* table) {
+    if (threadIdx.x < kTable) table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / kTable);
 }
+struct Weights {
+    const double* table;
+    float m;
+    double per_step;  // 32 log2(e) / T
 
-// A weight of [0, 1] as a multiple of 2^-43, rounded to nearest: the sum with 2^9 holds 2^-43 in its last bit.
-__device__ __forceinline__ u64 fixed(double w) {
-    return static_cast<u64>(__double_as_longlong(w + 512.0) - __double_as_longlong(512.0));
-}
+    __device__ __forceinline__ Weights(const double* table_, float m_, double per_t)
+        : table(table_), m(m_), per_step(per_t * (kTable * 1.44269504088896340736)) {}
 
-__device__ __forceinline__ u64 shuffle_up(u64 v, int by) { return __shfl_up(v, by, kWave); }
-
-// Inclusive prefix sum over a wave.
-__device__ __forceinline__ u64 wave_scan(u64 v) {
-    const int lane = threadIdx.x % kWave;
-#pragma unroll
-    for (int by = 1; by < kWave; by *= 2) {
-        const u64 o = shuffle_up(v, by);
-        if (lane >= by) v += o;
+    __device__ __forceinline__ u64 operator()(float z) const {
+        double t = (static_cast<double>(z) - static_cast<double>(m)) * per_step;
+        const bool counts = t > -46.0 * kTable;  // below, the weight rounds to 0; NaN is masked
+        t = counts ? t : 0.0;
+        const double n = __builtin_rint(t);
+        const double f = (t - n) * (0.693147180559945309417 / kTable);
+        const int i = static_cast<int>(n);
+        double e = __builtin_fma(f, 1.0 / 120, 1.0 / 24);
+        e = __builtin_fma(f, e, 1.0 / 6);
+        e = __builtin_fma(f, e, 0.5);
+        e = __builtin_fma(f, e, 1.0);
+        e = __builtin_fma(f, e, 1.0);
+        const double w = __builtin_ldexp(table[i & (kTable - 1)] * e, i >> 5);
+        // added to 2^9 a weight of [0, 1] is rounded to a multiple of 2^-43 in the sum's last bits
+        const u64 fixed = static_cast<u64>(__double_as_longlong(w + 512.0) - __double_as_longlong(512.0));
+        return z == m ? 1ULL << 43 : counts ? fixed : 0ULL;  // m itself, infinite or not, weighs 1
     }
-    return v;
-}
+};
 
+template <int Control>
+__device__ __forceinline__ u64 dpp64(u64 v) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), Control, 0xF, 0xF, true);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), Control, 0xF, 0xF, true);
+    return (static_cast<u64>(hi) << 32) | lo;
+}
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {
+    const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane);
+    const unsigned hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+    return (static_cast<u64>(hi) << 32) | lo;
+}
+// Sum over a wave, in every lane.
 __device__ __forceinline__ u64 wave_total(u64 v) {
+    v += dpp64<kDppXor1>(v);
+    v += dpp64<kDppXor2>(v);
+    v += dpp64<kDppHalfMirror>(v);
+    v += dpp64<kDppMirror>(v);
+    return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+}
+// Inclusive prefix sum over a wave: shifts by 1, 2, 4 and 8 inside the rows of 16 lanes, then the rows before.
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+    v += dpp64<0x111>(v);
+    v += dpp64<0x112>(v);
+    v += dpp64<0x114>(v);
+    v += dpp64<0x118>(v);
+    const u64 a = lane64(v, 15), b = a + lane64(v, 31), c = b + lane64(v, 47);
+    const int row = threadIdx.x % kWave / 16;
+    return v + (row == 0 ? 0 : row == 1 ? a : row == 2 ? b : c);
+}
+__device__ __forceinline__ int wave_scan(int v) { return static_cast<int>(wave_scan(static_cast<u64>(v))); }
+__device__ __forceinline__ int wave_total(int v) { return static_cast<int>(wave_total(static_cast<u64>(v))); }
+__device__ __forceinline__ unsigned wave_min(unsigned v) {
 #pragma unroll
-    for (int by = 32; by > 0; by /= 2) v += __shfl_xor(v, by, kWave);
+    for (int by = 32; by > 0; by /= 2) v = min(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), by, kWave)));
     return v;
 }
 
-template <int Group>
+__device__ __forceinline__ void nothing_drawn(const Params& p, long long r, bool valid) {
+    p.tokens[r] = -1;
+    if (p.log_probs) p.log_probs[r] = valid ? -INFINITY : NAN;
+}
+__device__ __forceinline__ void drawn(const Params& p, long long r, long long token, float z, float m, double per_t, u64 total) {
+    p.tokens[r] = token;
+    if (!p.log_probs) return;
+    const double x = z == m ? 0.0 : (static_cast<double>(z) - static_cast<double>(m)) * per_t;
+    p.log_probs[r] = static_cast<float>(x - log(static_cast<double>(total) / kScale));
+}
+
+// How many of the tokens of a border key stay (at most `ties`): the i-th does while the mass before it, above + i tie, is
+// below the border.
+__device__ __forceinline__ int ties_below(double border, u64 above, u64 tie, int ties) {
+    const double stay = ceil((border - static_cast<double>(above)) / static_cast<double>(tie));
+    return static_cast<int>(fmax(fmin(stay, static_cast<double>(ties)), 1.0));
+}
+
+// ---------------------------------------------------------------------------
+// Up to 1024 classes: one wave a row
+// ---------------------------------------------------------------------------
+constexpr int kRowsPerBlock = 4;
+
+template <typename T, int E>
+__global__ __launch_bounds__(kRowsPerBlock* kWave) void sample_wave(Params p) {
+    typedef typename T::Store Store;
+    // the bits of a key that 16-bit logits cannot differ in are dropped: fewer to bisect
+    constexpr int kShift = sizeof(Store) == 4 ? 0 : T::kNegInf == tokens::Bf16::kNegInf ? 16 : 13;
+    __shared__ double table[kTable];
+    fill_table(table);
+    __syncthreads();
+    const long long r = blockIdx.x * static_cast<long long>(kRowsPerBlock) + threadIdx.x / kWave;
+    if (r >= p.rows) return;
+    const int lane = threadIdx.x % kWave;
+    const Settings s(p, r);
+    const Store* row = static_cast<const Store*>(p.logits) + r * p.ld;
+    const int first = lane * E;
+    float z[E];
+    if (first + E <= p.classes) {
+        struct __attribute__((packed, aligned(sizeof(Store)))) Piece {
+            Store v[E];
+        };
+        const Piece piece = *reinterpret_cast<const Piece*>(row + first);
+#pragma unroll
+        for (int e = 0; e < E; ++e) z[e] = T::value(piece.v[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) z[e] = first + e < p.classes ? T::value(row[first + e]) : -INFINITY;
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmaxf(m, z[e]);
+    m = wave_max(m);
+    if (!s.valid || m == -INFINITY) {
+        if (lane == 0) nothing_drawn(p, r, s.valid);
+        return;
+    }
+    const Weights weight(table, m, s.per_t);
+    u64 w[E];
+    const bool cuts = s.one() || (s.top_k > 0 && s.top_k < p.classes) || s.top_p < 1.0;
+    if (!cuts) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = weight(z[e]);
+    } else {
+        unsigned key[E];  // 0: masked
+        const unsigned high = (ordered(m) >> kShift) + 1;
+        unsigned low = high;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            key[e] = masked(z[e]) ? 0 : (ordered(z[e]) >> kShift) + 1;
+            if (key[e]) low = min(low, key[e]);
+        }
+        low = wave_min(low);
+        // the largest key at which `reached` holds, which it does at `floor`; all keys lie in [low, high]
+        const auto bisect = [&](unsigned floor, auto reached) {
+            if (floor == high) return high;
+            int bit = 31 - __clz(floor ^ high);
+            unsigned border = high >> bit >> 1 << bit << 1;
+            for (; bit >= 0; --bit)
+                if (reached(border | (1u << bit))) border |= 1u << bit;
+            return border;
+        };
+        const auto count_from = [&](unsigned k) {
+            int n = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) n += __popcll(__ballot(key[e] >= k));
+            return n;
+        };
+        const auto mass_from = [&](unsigned k) {
+            u64 sum = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) sum += key[e] >= k ? w[e] : 0;
+            return wave_total(sum);
+        };
+        unsigned border = 0;  // keys above it stay, and the first `ties` of those equal to it
+        int ties = INT_MAX;
+        if (s.one()) {
+            border = high;
+            ties = 1;
+        } else if (s.top_k > 0 && s.top_k < count_from(1)) {
+            border = bisect(low, [&](unsigned k) { return count_from(k) >= s.top_k; });
+            ties = s.top_k - count_from(border + 1);
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) w[e] = s.one() ? (key[e] == high ? 1ULL << 43 : 0) : key[e] >= border ? weight(z[e]) : 0;
+        const auto weight_at = [&](unsigned k) {
+            u64 at = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const u64 found = __ballot(key[e] == k);
+                if (found) at = lane64(w[e], __ffsll(found) - 1);
+            }
+            return at;
+        };
+        if (s.top_p < 1.0 && !s.one()) {
+            const bool limited = ties != INT_MAX;
+            const u64 tie = limited ? weight_at(border) : 0;
+            const u64 above = mass_from(border + 1);
+            const double mass = s.top_p * static_cast<double>(above + (limited ? tie * static_cast<u64>(ties) : 0));
+            if (static_cast<double>(above) >= mass) {
+                border = bisect(max(border, low), [&](unsigned k) { return static_cast<double>(mass_from(k)) >= mass; });
+                ties = ties_below(mass, mass_from(border + 1), weight_at(border), p.classes);
+            } else if (tie > 0) {
+                ties = ties_below(mass, above, tie, ties);
+            }
+        }
+        int equal = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) equal += key[e] == border;
+        int rank = wave_scan(equal) - equal;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (key[e] < border || (key[e] == border && rank++ >= ties)) w[e] = 0;
+    }
+    u64 sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        w[e] = w[e] >= s.min_weight ? w[e] : 0;
+        sum += w[e];
+    }
+    const u64 upto = wave_scan(sum);
+    const u64 total = lane64(upto, kWave - 1);
+    const double target = s.target(total);
+    const u64 found = __ballot(static_cast<double>(upto) > target);
+    if (lane != __ffsll(found) - 1) return;
+    u64 run = upto - sum;
+    int at = -1;
+    float chosen = m;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        run += w[e];
+        if (at < 0 && static_cast<double>(run) > target) {
+            at = first + e;
+            chosen = z[e];
+        }
+    }
+    drawn(p, r, at, chosen, m, s.per_t, total);
+}
+
+// ---------------------------------------------------------------------------
+// Longer rows: one workgroup a row
+// ---------------------------------------------------------------------------
+constexpr int kBins = 1024;
+constexpr int kBinsPerLane = kBins / kWave;
+constexpr float kBinsPerUnit = 32.0f;  // linear bins of 1/32 of (max - z) / T: 32 units until the last one
+constexpr int kDigit = 10;             // bits of a digit: a bin each
+static_assert(kBins == 1 << kDigit, "a bin for each digit");
+constexpr int kCandidates = 1024;
+
 struct Shared {
     u64 bins[kBins];
+    u64 list[kCandidates];  // candidates of top-k: key, then ~index
+    double table[kTable];
     u64 above;      // running sum before the bin found
     double border;
-    int bin;
+    int bin, count;
     unsigned low, high;
-    float reduce[Team<Group>::kWaves];
+    float reduce[16];
+    u64 sums[16];
 };
 
 // Wave 0: the first bin, in order, at which the running sum reaches `border`; -1 if none does.  Leaves the sum before
@@ -110,32 +345,29 @@ __device__ __forceinline__ int find_bin(const u64* bins, u64 start, double borde
     const u64 upto = start + wave_scan(mine);
     const u64 found = __ballot(static_cast<double>(upto) >= border);
     if (!found) {
-        before = __shfl(upto, kWave - 1, kWave);
+        before = lane64(upto, kWave - 1);
         return -1;
     }
     const int first = __ffsll(found) - 1;
-    u64 sum = __shfl(upto - mine, first, kWave);
-    int bin = first * kBinsPerLane;
-    for (int i = 0; i < kBinsPerLane; ++i, ++bin) {
-        const u64 next = sum + bins[first * kBinsPerLane + i];
-        if (static_cast<double>(next) >= border) break;
-        sum = next;
-    }
-    before = sum;
-    return bin;
+    // the lane's bins, one a lane
+    const u64 start_here = lane64(upto - mine, first);
+    const u64 here = lane < kBinsPerLane ? bins[first * kBinsPerLane + lane] : 0;
+    const u64 sum = start_here + wave_scan(here);
+    const int at = __ffsll(__ballot(static_cast<double>(sum) >= border)) - 1;
+    before = lane64(sum - here, at);
+    return first * kBinsPerLane + at;
 }
 
-template <typename T, int Group, int Held>
+template <typename T, int Group, bool Held>
 struct Sampler {
     typedef Team<Group> G;
-    typedef Row<T, Group, Held> R;
+    typedef tokens::LongRow<T, Group, Held> R;
     static constexpr int V = T::kPerChunk;
 
     const R& row;
-    Shared<Group>& s;
+    Shared& s;
     const int t;
     const float m;         // the row's maximum
-    const double per_t;
     const float per_bin;   // bins of a unit of logits
 
     __device__ __forceinline__ int bin_of(float z) const {
@@ -149,23 +381,26 @@ struct Sampler {
         if (t == 0) {
             s.low = 0xffffffffu;
             s.high = 0;
+            s.count = 0;
         }
-        G::sync();
+        __syncthreads();
     }
 
     // The key, above `floor`, at which the running sum of f reaches border_of(sum of all): in `key`, with the sum of
     // the keys above it in `above`.  False if none does; `above` is then the sum of all.  The border must be positive.
+    // A histogram over the distance to the maximum, then digits of the keys in the bin in which the border lies, from
+    // the first bit in which they differ.
     template <typename F, typename B>
     __device__ __forceinline__ bool cut_at(F f, B border_of, unsigned floor, unsigned& key, u64& above) {
         clear_bins();
-        row.each([&](int, const float (&v)[V], int) {
+        row.each([&](const float (&v)[V], int) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 if (masked(v[e]) || ordered(v[e]) <= floor) continue;
                 atomicAdd(&s.bins[bin_of(v[e])], f(v[e]));
             }
         });
-        G::sync();
+        __syncthreads();
         if (t < kWave) {
             u64 all = 0;
 #pragma unroll
@@ -179,13 +414,12 @@ struct Sampler {
                 s.bin = bin;
             }
         }
-        G::sync();
+        __syncthreads();
         const int bin = s.bin;
         above = s.above;
         if (bin < 0) return false;
-        // the bin's keys: digits from the first bit in which they differ
         unsigned low = 0xffffffffu, high = 0;
-        row.each([&](int, const float (&v)[V], int) {
+        row.each([&](const float (&v)[V], int) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const unsigned k = ordered(v[e]);
@@ -198,25 +432,25 @@ struct Sampler {
             atomicMin(&s.low, low);
             atomicMax(&s.high, high);
         }
-        G::sync();
+        __syncthreads();
         low = s.low;
         high = s.high;
         unsigned prefix = low;  // the keys still searched agree with it above `bits`
         int bits = low == high ? 0 : 32 - __clz(low ^ high);
         while (bits > 0) {
             const int digit = min(bits, kDigit), shift = bits - digit;
-            G::sync();
+            __syncthreads();
             clear_bins();
-            row.each([&](int, const float (&v)[V], int) {
+            row.each([&](const float (&v)[V], int) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
                     const unsigned k = ordered(v[e]);
-                    if (masked(v[e]) || k <= floor || bin_of(v[e]) != bin) continue;
+                    if (k < low || k > high || masked(v[e])) continue;
                     if (bits < 32 && ((k ^ prefix) >> bits)) continue;
                     atomicAdd(&s.bins[kBins - 1 - ((k >> shift) & ((1u << digit) - 1))], f(v[e]));
                 }
             });
-            G::sync();
+            __syncthreads();
             if (t < kWave) {
                 u64 before;
                 const int found = find_bin(s.bins, s.above, s.border, before);
@@ -225,7 +459,7 @@ struct Sampler {
                     s.bin = found;
                 }
             }
-            G::sync();
+            __syncthreads();
             const unsigned value = static_cast<unsigned>(kBins - 1 - s.bin) & ((1u << digit) - 1);
             const unsigned mask = bits < 32 ? (1u << bits) - 1 : 0xffffffffu;
             prefix = (prefix & ~mask) | (value << shift);
@@ -235,120 +469,213 @@ struct Sampler {
         above = s.above;
         return true;
     }
+
+    // The first k of the order by way of a short list, where k is small: the k-th largest of the threads' maxima bounds
+    // the k-th largest of all from below, and few other values lie above it.  Leaves the list sorted, the order's first
+    // first, and returns its length; 0 if it came out too long.
+    __device__ __forceinline__ int shortlist(int k, float mine) {
+        clear_bins();
+        const int bin = masked(mine) ? kBins : bin_of(mine);
+        if (bin < kBins) atomicAdd(&s.bins[bin], 1ULL);
+        __syncthreads();
+        if (t < kWave) {
+            u64 before;
+            const int found = find_bin(s.bins, 0, static_cast<double>(k), before);
+            if (t == 0) s.bin = found;
+        }
+        __syncthreads();
+        if (s.bin < 0) return 0;  // fewer threads than k hold a value
+        if (bin <= s.bin) atomicMin(&s.low, ordered(mine));
+        __syncthreads();
+        const float least = from_ordered(s.low);
+        row.each_with(
+            [&](float top) { return top >= least; },
+            [&](const float (&v)[V], int first) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    if (!(v[e] >= least)) continue;
+                    const int at = atomicAdd(&s.count, 1);
+                    if (at < kCandidates) s.list[at] = (static_cast<u64>(ordered(v[e])) << 32) | ~static_cast<unsigned>(first + e);
+                }
+            });
+        __syncthreads();
+        const int count = s.count;
+        if (count > min(kCandidates, Group)) return 0;
+        sort(count);
+        return count;
+    }
+
+    // Descending bitonic sort of the list's first `count`, one a thread; partners within a wave exchange by shuffles.
+    __device__ __forceinline__ void sort(int count) {
+        int size = kWave;
+        while (size < count) size *= 2;
+        u64 x = t < count ? s.list[t] : 0;
+        __syncthreads();
+        if (t < size) {
+            for (int run = 2; run <= kWave; run *= 2)
+                for (int by = run / 2; by > 0; by /= 2) x = exchange(x, __shfl_xor(x, by, kWave), by, run);
+        }
+        for (int run = 2 * kWave; run <= size; run *= 2) {
+            for (int by = run / 2; by >= kWave; by /= 2) {
+                if (t < size) s.list[t] = x;
+                __syncthreads();
+                if (t < size) x = exchange(x, s.list[t ^ by], by, run);
+                __syncthreads();
+            }
+            if (t < size)
+                for (int by = kWave / 2; by > 0; by /= 2) x = exchange(x, __shfl_xor(x, by, kWave), by, run);
+        }
+        if (t < size) s.list[t] = x;
+        __syncthreads();
+    }
+    __device__ __forceinline__ u64 exchange(u64 x, u64 other, int by, int run) const {
+        const bool larger = ((t & run) == 0) == ((t & by) == 0);
+        return (x > other) == larger ? x : other;
+    }
+
+    // Inclusive prefix sum over the workgroup's threads.
+    __device__ __forceinline__ u64 scan(u64 v) {
+        v = wave_scan(v);
+        if (t % kWave == kWave - 1) s.sums[t / kWave] = v;
+        __syncthreads();
+        for (int i = 0; i < t / kWave; ++i) v += s.sums[i];
+        return v;
+    }
 };
 
-// The logit whose ordered bits are `key`.
-__device__ __forceinline__ float from_ordered(unsigned key) {
-    return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
-}
-
-template <typename T, int Group, int Held, int Segments>
-__global__ __launch_bounds__(Group < 256 ? 256 : Group) void sample_kernel(Params p) {
+template <typename T, int Group, bool Held, int Segments>
+__global__ __launch_bounds__(Group) void sample_block(Params p) {
     typedef typename T::Store Store;
     typedef Team<Group> G;
-    constexpr int kTeams = Group < 256 ? 256 / Group : 1;
     constexpr int V = T::kPerChunk;
-    __shared__ Shared<Group> shared[kTeams];
-    __shared__ u64 segment_mass[kTeams][Segments];
-    __shared__ int segment_ties[kTeams][Segments];
-    const int team = static_cast<int>(threadIdx.x) / Group % kTeams;
-    Shared<Group>& s = shared[team];
-    u64* mass = segment_mass[team];
-    int* tied = segment_ties[team];
+    __shared__ Shared s;
+    __shared__ u64 mass[Segments];
+    __shared__ int tied[Segments];
+    fill_table(s.table);
+    const long long r = blockIdx.x;
+    const int t = static_cast<int>(threadIdx.x), lane = t % kWave;
+    const Settings set(p, r);
 
-    const long long r = blockIdx.x * static_cast<long long>(kTeams) + threadIdx.x / Group;
-    if (r >= p.rows) return;  // a team of its own wave, or none of the workgroup
-    const int t = G::thread(), lane = t % kWave;
-    const double temperature = p.temperatures ? p.temperatures[r] : p.temperature;
-    const double top_p = p.top_ps ? p.top_ps[r] : p.top_p;
-    const double min_p = fmin(p.min_ps ? p.min_ps[r] : p.min_p, 1.0);
-    const int top_k = p.top_ks ? p.top_ks[r] : p.top_k;
-    const float u = p.uniform[r];
-    const bool valid = temperature >= 0.0 && temperature < INFINITY && top_p == top_p &&
-                       (p.min_ps ? p.min_ps[r] == p.min_ps[r] : true) && u == u;
-
-    Row<T, Group, Held> row;
+    tokens::LongRow<T, Group, Held> row;
     row.open(static_cast<const Store*>(p.logits) + r * p.ld, p.classes);
-    float m = -INFINITY;
-    row.each([&](int, const float (&v)[V], int) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) m = fmaxf(m, v[e]);
-    });
-    m = G::max(m, s.reduce);
-    if (!valid || m == -INFINITY) {
-        if (t == 0) {
-            p.tokens[r] = -1;
-            if (p.log_probs) p.log_probs[r] = valid ? -INFINITY : NAN;
-        }
+    float mine = -INFINITY;
+    row.each_max([&](float top) { mine = fmaxf(mine, top); });
+    const float m = G::max(mine, s.reduce);
+    if (!set.valid || m == -INFINITY) {
+        if (t == 0) nothing_drawn(p, r, set.valid);
         return;
     }
-    const bool greedy = temperature == 0.0;
-    const double per_t = greedy ? 0.0 : 1.0 / temperature;
-    const float per_bin = static_cast<float>(kBinsPerUnit * per_t);
-    Sampler<T, Group, Held> sampler{row, s, t, m, per_t, per_bin};
+    const Weights weight(s.table, m, set.per_t);
+    Sampler<T, Group, Held> sampler{row, s, t, m, static_cast<float>(kBinsPerUnit * set.per_t)};
 
     // what stays of the order: keys above `key`, and the first `ties` (by index) of those equal to it
     unsigned key = 0;
     int ties = INT_MAX;
-    if (greedy || top_p <= 0.0 || top_k == 1) {
+    if (set.one()) {
         key = ordered(m);
         ties = 1;
     } else {
         unsigned cut;
         u64 above;
-        if (top_k > 0 && top_k < p.classes &&
-            sampler.cut_at([](float) { return 1ULL; }, [&](u64) { return static_cast<double>(top_k); }, 0u, cut, above)) {
-            key = cut;
-            ties = top_k - static_cast<int>(above);
-        }
-        if (top_p < 1.0) {
-            G::sync();
-            const bool limited = ties != INT_MAX;
-            u64 tie = limited ? fixed(weight(from_ordered(key), m, per_t)) : 0;
-            const u64 tied = limited ? tie * static_cast<u64>(ties) : 0;
-            const bool found = sampler.cut_at([&](float z) { return fixed(weight(z, m, per_t)); },
-                                              [&](u64 all) { return top_p * static_cast<double>(all + tied); },
-                                              limited ? key : 0u, cut, above);
-            if (found) {
-                key = cut;
-                tie = fixed(weight(from_ordered(key), m, per_t));
-                ties = p.classes;
+        const bool top_k = set.top_k > 0 && set.top_k < p.classes;
+        const int listed = top_k && set.top_k <= Group / 2 ? sampler.shortlist(set.top_k, mine) : 0;
+        if (listed) {
+            // the list holds the order's first `listed`: weights and borders from there
+            const u64 entry = t < listed ? s.list[t] : 0;
+            const unsigned own = static_cast<unsigned>(entry >> 32);
+            u64 w = t < min(set.top_k, listed) ? weight(from_ordered(own)) : 0;
+            const u64 upto = sampler.scan(w);
+            __syncthreads();
+            if (t == Group - 1) s.above = upto;
+            if (t == 0) s.count = 0;
+            __syncthreads();
+            const double border = set.top_p < 1.0 ? set.top_p * static_cast<double>(s.above) : INFINITY;
+            const bool stays = t < min(set.top_k, listed) &&
+                               (t == 0 || (static_cast<double>(upto - w) < border && w >= set.min_weight));
+            const u64 votes = __ballot(stays);
+            if (lane == 0 && votes) atomicAdd(&s.count, __popcll(votes));
+            __syncthreads();
+            const int kept = s.count;
+            if (kept <= kWave) {
+                // wave 0 has them all: the running sums by index
+                if (t >= kWave) return;
+                w = t < kept ? w : 0;
+                const unsigned index = ~static_cast<unsigned>(entry);
+                u64 run = 0, total = 0;
+                for (int i = 0; i < kept; ++i) {
+                    const u64 other = lane64(w, i);
+                    total += other;
+                    run += static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(index), i)) <= index ? other : 0;
+                }
+                const double target = set.target(total);
+                // of those whose running sum passes the target the one of the lowest index
+                const unsigned first = wave_min(t < kept && static_cast<double>(run) > target ? index : 0xffffffffu);
+                if (t < kept && index == first) drawn(p, r, index, from_ordered(own), m, set.per_t, total);
+                return;
             }
-            // the i-th of the equal keys stays while the mass before it, above + i tie, is below the border
-            if ((found || limited) && tie > 0) {
-                const double stay = ceil((s.border - static_cast<double>(above)) / static_cast<double>(tie));
-                ties = static_cast<int>(fmax(fmin(stay, static_cast<double>(ties)), 1.0));
+            __syncthreads();
+            if (t == kept - 1) s.low = own;
+            if (t == 0) s.count = 0;
+            __syncthreads();
+            key = s.low;
+            const u64 equal = __ballot(t < kept && own == key);
+            if (lane == 0 && equal) atomicAdd(&s.count, __popcll(equal));
+            __syncthreads();
+            ties = s.count;
+        } else {
+            if (top_k) __syncthreads();
+            if (top_k && sampler.cut_at([](float) { return 1ULL; }, [&](u64) { return static_cast<double>(set.top_k); }, 0u,
+                                        cut, above)) {
+                key = cut;
+                ties = set.top_k - static_cast<int>(above);
+            }
+            if (set.top_p < 1.0) {
+                __syncthreads();
+                const bool limited = ties != INT_MAX;
+                u64 tie = limited ? weight(from_ordered(key)) : 0;
+                const u64 tied_mass = limited ? tie * static_cast<u64>(ties) : 0;
+                const bool found = sampler.cut_at([&](float z) { return weight(z); },
+                                                  [&](u64 all) { return set.top_p * static_cast<double>(all + tied_mass); },
+                                                  limited ? key : 0u, cut, above);
+                if (found) {
+                    key = cut;
+                    tie = weight(from_ordered(key));
+                    ties = p.classes;
+                }
+                if ((found || limited) && tie > 0) ties = ties_below(s.border, above, tie, ties);
             }
         }
     }
-    const double tie_weight = ties == INT_MAX ? 0.0 : weight(from_ordered(key), m, per_t);
-    const u64 tie = tie_weight >= min_p ? fixed(tie_weight) : 0;
+    const float least = key ? from_ordered(key) : -FLT_MAX;
+    u64 tie = ties == INT_MAX ? 0 : weight(least);
+    if (tie < set.min_weight) tie = 0;
 
     // kept mass (without ties) and ties of every segment of 64 chunks, in index order
     const auto kept = [&](float z) -> u64 {
-        if (masked(z) || ordered(z) <= key) return 0;
-        const double w = weight(z, m, per_t);
-        return w >= min_p ? fixed(w) : 0;
+        const u64 w = weight(z);
+        return (ties == INT_MAX ? z >= least : z > least) && w >= set.min_weight ? w : 0;
     };
-    const auto is_tie = [&](float z) { return !masked(z) && ordered(z) == key; };
+    const auto is_tie = [&](float z) { return ties != INT_MAX && z == least; };
     const int segments = row.passes() * G::kWaves;
-    row.each([&](int i, const float (&v)[V], int) {
-        if (i >= row.passes()) return;
+    row.each_pass([&](int i, const float (&v)[V], float top) {
         u64 sum = 0;
         int equal = 0;
+        if (__ballot(top >= least)) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            sum += kept(v[e]);
-            equal += is_tie(v[e]);
+            for (int e = 0; e < V; ++e) {
+                if (__ballot(v[e] >= least) == 0) continue;
+                sum += kept(v[e]);
+                equal += is_tie(v[e]);
+            }
+            sum = wave_total(sum);
+            if (ties != INT_MAX) equal = wave_total(equal);
         }
-        sum = wave_total(sum);
-        equal = static_cast<int>(wave_total(static_cast<u64>(equal)));
         if (lane == 0) {
             mass[i * G::kWaves + G::wave()] = sum;
             tied[i * G::kWaves + G::wave()] = equal;
         }
     });
-    G::sync();
+    __syncthreads();
     if (t >= kWave) return;
 
     // wave 0: the ties that stay in each segment, the sum of all, and the segment where it passes u
@@ -357,7 +684,7 @@ __global__ __launch_bounds__(Group < 256 ? 256 : Group) void sample_kernel(Param
     for (int first = 0; first < segments; first += kWave) {
         const int g = first + lane;
         const int equal = g < segments ? tied[g] : 0;
-        const int upto = ties_before + static_cast<int>(wave_scan(static_cast<u64>(equal)));
+        const int upto = ties_before + wave_scan(equal);
         const int before = upto - equal;
         u64 sum = 0;
         if (g < segments) {
@@ -366,10 +693,10 @@ __global__ __launch_bounds__(Group < 256 ? 256 : Group) void sample_kernel(Param
             tied[g] = before;
         }
         total += wave_total(sum);
-        ties_before = __shfl(upto, kWave - 1, kWave);
+        ties_before = __builtin_amdgcn_readlane(upto, kWave - 1);
     }
     Team<kWave>::sync();
-    const double target = fmax(fmin(static_cast<double>(u), 1.0 - 0x1p-50), 0.0) * static_cast<double>(total);
+    const double target = set.target(total);
     u64 before = 0;
     int segment = -1;
     for (int first = 0; first < segments && segment < 0; first += kWave) {
@@ -380,9 +707,9 @@ __global__ __launch_bounds__(Group < 256 ? 256 : Group) void sample_kernel(Param
         if (found) {
             const int at = __ffsll(found) - 1;
             segment = first + at;
-            before = __shfl(upto - sum, at, kWave);
+            before = lane64(upto - sum, at);
         } else {
-            before = __shfl(upto, kWave - 1, kWave);
+            before = lane64(upto, kWave - 1);
         }
     }
 
@@ -393,7 +720,7 @@ __global__ __launch_bounds__(Group < 256 ? 256 : Group) void sample_kernel(Param
     int equal = 0;
 #pragma unroll
     for (int e = 0; e < V; ++e) equal += is_tie(v[e]);
-    int rank = tied[segment] + static_cast<int>(wave_scan(static_cast<u64>(equal))) - equal;
+    int rank = tied[segment] + wave_scan(equal) - equal;
     u64 w[V], sum = 0;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -404,27 +731,42 @@ __global__ __launch_bounds__(Group < 256 ? 256 : Group) void sample_kernel(Param
     const u64 found = __ballot(static_cast<double>(upto) > target);
     if (lane != __ffsll(found) - 1) return;
     u64 run = upto - sum;
-    bool done = false;
+    int at = -1;
+    float chosen = m;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         run += w[e];
-        if (done || !(static_cast<double>(run) > target)) continue;
-        done = true;
-        p.tokens[r] = static_cast<long long>(chunk) * V + e;
-        if (p.log_probs) {
-            const double x = v[e] == m ? 0.0 : (static_cast<double>(v[e]) - static_cast<double>(m)) * per_t;
-            p.log_probs[r] = static_cast<float>(x - log(static_cast<double>(total) * 0x1p-43));
+        if (at < 0 && static_cast<double>(run) > target) {
+            at = chunk * V + e;
+            chosen = v[e];
         }
     }
+    drawn(p, r, at, chosen, m, set.per_t, total);
+}
+
+template <typename T, int E>
+void launch_wave(const Params& p, hipStream_t stream) {
+    hipLaunchKernelGGL((sample_wave<T, E>), dim3(ceil_div(p.rows, kRowsPerBlock)), dim3(kRowsPerBlock * kWave), 0, stream, p);
+}
+
+template <typename T, int Group, bool Held>
+void launch_block(const Params& p, hipStream_t stream) {
+    constexpr int kSegments = Held ? tokens::kHeldChunks * Group / kWave : kMaxClasses / (kWave * T::kPerChunk);
+    hipLaunchKernelGGL((sample_block<T, Group, Held, kSegments>), dim3(static_cast<unsigned>(p.rows)), dim3(Group), 0, stream,
+                       p);
 }
 
 template <typename T>
 void launch(const Params& p, hipStream_t stream) {
-    if (p.classes <= 64 * T::kPerChunk)
-        hipLaunchKernelGGL((sample_kernel<T, 64, 1, 1>), dim3(ceil_div(p.rows, 4)), dim3(256), 0, stream, p);
-    else
-        hipLaunchKernelGGL((sample_kernel<T, 256, 0, kMaxClasses / (64 * T::kPerChunk)>),
-                           dim3(static_cast<unsigned>(p.rows)), dim3(256), 0, stream, p);
+    constexpr int kHeld = tokens::kHeldChunks * T::kPerChunk;  // classes a thread can hold
+    if (p.classes <= 64) launch_wave<T, 1>(p, stream);
+    else if (p.classes <= 128) launch_wave<T, 2>(p, stream);
+    else if (p.classes <= 256) launch_wave<T, 4>(p, stream);
+    else if (p.classes <= 512) launch_wave<T, 8>(p, stream);
+    else if (p.classes <= 1024) launch_wave<T, 16>(p, stream);
+    else if (p.classes <= 256 * kHeld && (p.rows > 512 || p.classes <= 4096)) launch_block<T, 256, true>(p, stream);
+    else if (p.classes <= 1024 * kHeld) launch_block<T, 1024, true>(p, stream);
+    else launch_block<T, 1024, false>(p, stream);
 }
 
 }  // namespace sample

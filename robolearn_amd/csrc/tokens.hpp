@@ -207,5 +207,104 @@ struct Row {
     }
 };
 
+// A long row over a whole workgroup: as Row, but the passes run in loops.  Held: the row lives in the registers of the
+// group (up to kHeldChunks chunks a thread, four vectors that a loop indexes by one scalar); unrolled over 16 chunks the
+// passes over it would not fit the instruction cache.  Else every pass reads memory again.
+constexpr int kHeldChunks = 16;
+
+template <typename T, int Group, bool Held>
+struct LongRow {
+    typedef typename T::Store Store;
+    typedef unsigned Words __attribute__((ext_vector_type(kHeldChunks)));
+    static constexpr int V = T::kPerChunk;
+    Row<T, Group, 0> memory;
+    Words x, y, z, w;
+
+    __device__ __forceinline__ void open(const Store* row, int classes) {
+        memory.open(row, classes);
+        if constexpr (Held) {
+            const int t = static_cast<int>(threadIdx.x);
+#pragma unroll
+            for (int i = 0; i < kHeldChunks; ++i) {
+                const int c = t + i * Group;
+                const uint4 q = c < memory.full ? memory.load(c) : memory.nothing();
+                x[i] = q.x, y[i] = q.y, z[i] = q.z, w[i] = q.w;
+            }
+            if (memory.rest && t == memory.full % Group) {
+                const uint4 q = memory.load_rest();
+                const int last = memory.full / Group;
+#pragma unroll
+                for (int i = 0; i < kHeldChunks; ++i)
+                    if (i == last) x[i] = q.x, y[i] = q.y, z[i] = q.z, w[i] = q.w;
+            }
+        }
+    }
+    __device__ __forceinline__ int passes() const { return memory.passes(); }
+    __device__ __forceinline__ uint4 read(int c) const { return memory.read(c); }
+    __device__ __forceinline__ uint4 chunk(int i) const {
+        if constexpr (Held) return make_uint4(x[i], y[i], z[i], w[i]);
+        else return memory.chunk(i);
+    }
+    __device__ __forceinline__ static float top_of(const float (&v)[V]) {
+        float top = v[0];
+#pragma unroll
+        for (int e = 1; e < V; ++e) top = fmaxf(top, v[e]);
+        return top;
+    }
+    // f(i, values, their maximum) for every pass
+    template <typename F>
+    __device__ __forceinline__ void each_pass(F f) const {
+        const int n = passes();
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            float v[V];
+            T::unpack(chunk(i), v);
+            f(i, v, top_of(v));
+        }
+    }
+    // f(values, index of the first)
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+        const int n = passes();
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            float v[V];
+            T::unpack(chunk(i), v);
+            f(v, (static_cast<int>(threadIdx.x) + i * Group) * V);
+        }
+    }
+    // the same where wanted(maximum) holds
+    template <typename W, typename F>
+    __device__ __forceinline__ void each_with(W wanted, F f) const {
+        const int n = passes();
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            float v[V];
+            T::unpack(chunk(i), v);
+            if (wanted(top_of(v))) f(v, (static_cast<int>(threadIdx.x) + i * Group) * V);
+        }
+    }
+    // f(maximum of the chunk)
+    template <typename F>
+    __device__ __forceinline__ void each_max(F f) const {
+        const int n = passes();
+        if constexpr (Held) {
+#pragma unroll
+            for (int i = 0; i < kHeldChunks; ++i) {
+                float v[V];
+                T::unpack(chunk(i), v);
+                f(top_of(v));
+            }
+        } else {
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+                float v[V];
+                T::unpack(chunk(i), v);
+                f(top_of(v));
+            }
+        }
+    }
+};
+
 }  // namespace tokens
 }  // namespace rl
