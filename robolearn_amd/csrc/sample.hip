@@ -14,8 +14,8 @@
 // LDS atomics and sums over waves in any order give the same token on every run.
 //
 // No row is sorted.  A cut of the order (top-k by counts, top-p by mass) is a border key (the order-preserving bits of
-// the logits) and how many tokens of exactly that key stay, by index.  Rows of up to 1024 classes: one wave a row, E
-// consecutive classes a lane, the border by bisection of the key's bits.  Longer rows: one workgroup a row, in registers
+// the logits) and how many tokens of exactly that key stay, by index.  Rows of up to 1024 classes: 16 or 64
+// lanes a row, the border by bisection of the key's bits.  Longer rows: one workgroup a row, in registers
 // where they fit, with the paths below.
 #include "tokens.hpp"
 
@@ -85,7 +85,7 @@ __device__ __forceinline__ bool masked(float z) { return !(z > -INFINITY); }  //
 
 // exp((z - m) / T) as a multiple of 2^-43.  With t = (z - m) 32 log2(e) / T = 32 e + i + f, |f| <= 1/2, it is 2^e times
 // 2^(i / 32), from a table of 32 (one LDS bank pair each), times the Taylor sum of exp(f ln2 / 32) to the fifth order, which
-// leaves (ln2 / 64)^6 / 720 = 2e-15 of it.  17 instructions against about 45 of exp().
+// leaves (ln2 / 64)^6 / 720 = 2e-15 of it: 20 instructions where exp() takes about 45.
 constexpr int kTable = 32;
 __device__ __forceinline__ void fill_table(double* table) {
     if (threadIdx.x < kTable) table[threadIdx.x] = exp2(static_cast<double>(threadIdx.x) / kTable);
@@ -94,33 +94,57 @@ struct Weights {
     const double* table;
     float m;
     double per_step;  // 32 log2(e) / T
+    bool alone;       // only m itself weighs anything: an infinite maximum, or 1 / T past the doubles
 
     __device__ __forceinline__ Weights(const double* table_, float m_, double per_t)
-        : table(table_), m(m_), per_step(per_t * (kTable * 1.44269504088896340736)) {}
+        : table(table_), m(m_), per_step(per_t * (kTable * 1.44269504088896340736)) {
+        alone = !(m < INFINITY) || !(per_step < INFINITY);
+    }
 
+    template <int N>
+    __device__ __forceinline__ void operator()(const float (&z)[N], u64 (&w)[N]) const {
+        if (alone) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = z[e] == m ? 1ULL << 43 : 0;
+            return;
+        }
+        constexpr double kRound = 0x1.8p52;  // added and taken off again: the nearest whole number, whose bits end the sum
+        constexpr double kStep = 0.693147180559945309417 / kTable;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            double t = (static_cast<double>(z[e]) - static_cast<double>(m)) * per_step;
+            t = __builtin_fmax(t, -46.0 * kTable);  // rounds to weight 0, as NaN does
+            const double sum = t + kRound;
+            const double f = t - (sum - kRound);
+            const int n = static_cast<int>(__double_as_longlong(sum));
+            double x = __builtin_fma(f, kStep * kStep * kStep * kStep * kStep / 120, kStep * kStep * kStep * kStep / 24);
+            x = __builtin_fma(f, x, kStep * kStep * kStep / 6);
+            x = __builtin_fma(f, x, kStep * kStep / 2);
+            x = __builtin_fma(f, x, kStep);
+            x = __builtin_fma(f, x, 1.0);
+            x *= table[n & (kTable - 1)];
+            // times 2^(n >> 5); x lies in [0.98, 2), the power above 2^-47
+            const u64 power = static_cast<u64>(static_cast<unsigned>(n >> 5) << 20) << 32;
+            x = __longlong_as_double(__double_as_longlong(x) + static_cast<long long>(power));
+            // added to 2^9 a weight of [0, 1] is rounded to a multiple of 2^-43 in the sum's last bits
+            w[e] = static_cast<u64>(__double_as_longlong(x + 512.0) - __double_as_longlong(512.0));
+        }
+    }
     __device__ __forceinline__ u64 operator()(float z) const {
-        double t = (static_cast<double>(z) - static_cast<double>(m)) * per_step;
-        const bool counts = t > -46.0 * kTable;  // below, the weight rounds to 0; NaN is masked
-        t = counts ? t : 0.0;
-        const double n = __builtin_rint(t);
-        const double f = (t - n) * (0.693147180559945309417 / kTable);
-        const int i = static_cast<int>(n);
-        double e = __builtin_fma(f, 1.0 / 120, 1.0 / 24);
-        e = __builtin_fma(f, e, 1.0 / 6);
-        e = __builtin_fma(f, e, 0.5);
-        e = __builtin_fma(f, e, 1.0);
-        e = __builtin_fma(f, e, 1.0);
-        const double w = __builtin_ldexp(table[i & (kTable - 1)] * e, i >> 5);
-        // added to 2^9 a weight of [0, 1] is rounded to a multiple of 2^-43 in the sum's last bits
-        const u64 fixed = static_cast<u64>(__double_as_longlong(w + 512.0) - __double_as_longlong(512.0));
-        return z == m ? 1ULL << 43 : counts ? fixed : 0ULL;  // m itself, infinite or not, weighs 1
+        const float v[1] = {z};
+        u64 w[1];
+        (*this)(v, w);
+        return w[0];
     }
 };
 
 template <int Control>
+__device__ __forceinline__ int dpp32(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, Control, 0xF, 0xF, true);
+}
+template <int Control>
 __device__ __forceinline__ u64 dpp64(u64 v) {
-    const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), Control, 0xF, 0xF, true);
-    const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), Control, 0xF, 0xF, true);
+    const unsigned lo = dpp32<Control>(static_cast<int>(v)), hi = dpp32<Control>(static_cast<int>(v >> 32));
     return (static_cast<u64>(hi) << 32) | lo;
 }
 __device__ __forceinline__ u64 lane64(u64 v, int lane) {
@@ -173,21 +197,72 @@ __device__ __forceinline__ int ties_below(double border, u64 above, u64 tie, int
 }
 
 // ---------------------------------------------------------------------------
-// Up to 1024 classes: one wave a row
+// Up to 1024 classes: Lanes lanes a row (16: four rows a wave share its instructions), E consecutive classes a lane
 // ---------------------------------------------------------------------------
-constexpr int kRowsPerBlock = 4;
+constexpr int kShortThreads = 256;
 
-template <typename T, int E>
-__global__ __launch_bounds__(kRowsPerBlock* kWave) void sample_wave(Params p) {
+template <int Lanes>
+struct Lane {
+    static_assert(Lanes == 16 || Lanes == kWave, "a row of lanes or a wave");
+    __device__ __forceinline__ static u64 total(u64 v) {
+        if constexpr (Lanes == kWave) return wave_total(v);
+        v += dpp64<kDppXor1>(v);
+        v += dpp64<kDppXor2>(v);
+        v += dpp64<kDppHalfMirror>(v);
+        return v + dpp64<kDppMirror>(v);
+    }
+    __device__ __forceinline__ static u64 scan(u64 v) {
+        if constexpr (Lanes == kWave) return wave_scan(v);
+        v += dpp64<0x111>(v);
+        v += dpp64<0x112>(v);
+        v += dpp64<0x114>(v);
+        return v + dpp64<0x118>(v);
+    }
+    __device__ __forceinline__ static int total(int v) {
+        v += dpp32<kDppXor1>(v);
+        v += dpp32<kDppXor2>(v);
+        v += dpp32<kDppHalfMirror>(v);
+        v += dpp32<kDppMirror>(v);
+        if constexpr (Lanes == kWave)
+            v = __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+                __builtin_amdgcn_readlane(v, 48);
+        return v;
+    }
+    __device__ __forceinline__ static int scan(int v) { return static_cast<int>(scan(static_cast<u64>(v))); }
+    __device__ __forceinline__ static float max(float v) {
+        if constexpr (Lanes == kWave) return wave_max(v);
+        v = fmaxf(v, dpp<kDppXor1>(v));
+        v = fmaxf(v, dpp<kDppXor2>(v));
+        v = fmaxf(v, dpp<kDppHalfMirror>(v));
+        return fmaxf(v, dpp<kDppMirror>(v));
+    }
+    __device__ __forceinline__ static unsigned max(unsigned v) {
+        v = ::max(v, static_cast<unsigned>(dpp32<kDppXor1>(static_cast<int>(v))));
+        v = ::max(v, static_cast<unsigned>(dpp32<kDppXor2>(static_cast<int>(v))));
+        v = ::max(v, static_cast<unsigned>(dpp32<kDppHalfMirror>(static_cast<int>(v))));
+        v = ::max(v, static_cast<unsigned>(dpp32<kDppMirror>(static_cast<int>(v))));
+        if constexpr (Lanes == kWave) {
+            const unsigned a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+            const unsigned c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+            v = ::max(::max(a, b), ::max(c, d));
+        }
+        return v;
+    }
+};
+
+template <typename T, int Lanes, int E>
+__global__ __launch_bounds__(kShortThreads) void sample_short(Params p) {
     typedef typename T::Store Store;
+    typedef Lane<Lanes> L;
+    constexpr int kRows = kShortThreads / Lanes;
     // the bits of a key that 16-bit logits cannot differ in are dropped: fewer to bisect
-    constexpr int kShift = sizeof(Store) == 4 ? 0 : T::kNegInf == tokens::Bf16::kNegInf ? 16 : 13;
+    constexpr int kShift = T::kKeyShift;
     __shared__ double table[kTable];
     fill_table(table);
     __syncthreads();
-    const long long r = blockIdx.x * static_cast<long long>(kRowsPerBlock) + threadIdx.x / kWave;
+    const long long r = blockIdx.x * static_cast<long long>(kRows) + threadIdx.x / Lanes;
     if (r >= p.rows) return;
-    const int lane = threadIdx.x % kWave;
+    const int lane = threadIdx.x % Lanes;
     const Settings s(p, r);
     const Store* row = static_cast<const Store*>(p.logits) + r * p.ld;
     const int first = lane * E;
@@ -206,27 +281,24 @@ __global__ __launch_bounds__(kRowsPerBlock* kWave) void sample_wave(Params p) {
     float m = -INFINITY;
 #pragma unroll
     for (int e = 0; e < E; ++e) m = fmaxf(m, z[e]);
-    m = wave_max(m);
+    m = L::max(m);
     if (!s.valid || m == -INFINITY) {
         if (lane == 0) nothing_drawn(p, r, s.valid);
         return;
     }
     const Weights weight(table, m, s.per_t);
     u64 w[E];
-    const bool cuts = s.one() || (s.top_k > 0 && s.top_k < p.classes) || s.top_p < 1.0;
-    if (!cuts) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = weight(z[e]);
-    } else {
+    weight(z, w);
+    if (s.one() || (s.top_k > 0 && s.top_k < p.classes) || s.top_p < 1.0) {
         unsigned key[E];  // 0: masked
         const unsigned high = (ordered(m) >> kShift) + 1;
-        unsigned low = high;
+        unsigned far = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             key[e] = masked(z[e]) ? 0 : (ordered(z[e]) >> kShift) + 1;
-            if (key[e]) low = min(low, key[e]);
+            if (key[e]) far = max(far, high - key[e]);
         }
-        low = wave_min(low);
+        const unsigned low = high - L::max(far);
         // the largest key at which `reached` holds, which it does at `floor`; all keys lie in [low, high]
         const auto bisect = [&](unsigned floor, auto reached) {
             if (floor == high) return high;
@@ -239,51 +311,52 @@ __global__ __launch_bounds__(kRowsPerBlock* kWave) void sample_wave(Params p) {
         const auto count_from = [&](unsigned k) {
             int n = 0;
 #pragma unroll
-            for (int e = 0; e < E; ++e) n += __popcll(__ballot(key[e] >= k));
-            return n;
+            for (int e = 0; e < E; ++e) n += key[e] >= k;
+            return L::total(n);
         };
         const auto mass_from = [&](unsigned k) {
             u64 sum = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) sum += key[e] >= k ? w[e] : 0;
-            return wave_total(sum);
+            return L::total(sum);
         };
-        unsigned border = 0;  // keys above it stay, and the first `ties` of those equal to it
+        // what a token of key k weighs (the key occurs)
+        const auto weight_at = [&](unsigned k) {
+            unsigned lo = 0, hi = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                lo = key[e] == k ? static_cast<unsigned>(w[e]) : lo;
+                hi = key[e] == k ? static_cast<unsigned>(w[e] >> 32) : hi;
+            }
+            return (static_cast<u64>(L::max(hi)) << 32) | L::max(lo);
+        };
+        unsigned border = 1;  // keys above it stay, and the first `ties` of those equal to it
         int ties = INT_MAX;
         if (s.one()) {
             border = high;
             ties = 1;
-        } else if (s.top_k > 0 && s.top_k < count_from(1)) {
-            border = bisect(low, [&](unsigned k) { return count_from(k) >= s.top_k; });
-            ties = s.top_k - count_from(border + 1);
-        }
-#pragma unroll
-        for (int e = 0; e < E; ++e) w[e] = s.one() ? (key[e] == high ? 1ULL << 43 : 0) : key[e] >= border ? weight(z[e]) : 0;
-        const auto weight_at = [&](unsigned k) {
-            u64 at = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const u64 found = __ballot(key[e] == k);
-                if (found) at = lane64(w[e], __ffsll(found) - 1);
+        } else {
+            if (s.top_k > 0 && s.top_k < count_from(1)) {
+                border = bisect(low, [&](unsigned k) { return count_from(k) >= s.top_k; });
+                ties = s.top_k - count_from(border + 1);
             }
-            return at;
-        };
-        if (s.top_p < 1.0 && !s.one()) {
-            const bool limited = ties != INT_MAX;
-            const u64 tie = limited ? weight_at(border) : 0;
-            const u64 above = mass_from(border + 1);
-            const double mass = s.top_p * static_cast<double>(above + (limited ? tie * static_cast<u64>(ties) : 0));
-            if (static_cast<double>(above) >= mass) {
-                border = bisect(max(border, low), [&](unsigned k) { return static_cast<double>(mass_from(k)) >= mass; });
-                ties = ties_below(mass, mass_from(border + 1), weight_at(border), p.classes);
-            } else if (tie > 0) {
-                ties = ties_below(mass, above, tie, ties);
+            if (s.top_p < 1.0) {
+                const bool limited = ties != INT_MAX;
+                const u64 tie = limited ? weight_at(border) : 0;
+                const u64 above = mass_from(limited ? border + 1 : 1);
+                const double mass = s.top_p * static_cast<double>(above + (limited ? tie * static_cast<u64>(ties) : 0));
+                if (static_cast<double>(above) >= mass) {
+                    border = bisect(max(border, low), [&](unsigned k) { return static_cast<double>(mass_from(k)) >= mass; });
+                    ties = ties_below(mass, mass_from(border + 1), weight_at(border), p.classes);
+                } else if (tie > 0) {
+                    ties = ties_below(mass, above, tie, ties);
+                }
             }
         }
         int equal = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) equal += key[e] == border;
-        int rank = wave_scan(equal) - equal;
+        int rank = L::scan(equal) - equal;
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (key[e] < border || (key[e] == border && rank++ >= ties)) w[e] = 0;
@@ -294,11 +367,10 @@ __global__ __launch_bounds__(kRowsPerBlock* kWave) void sample_wave(Params p) {
         w[e] = w[e] >= s.min_weight ? w[e] : 0;
         sum += w[e];
     }
-    const u64 upto = wave_scan(sum);
-    const u64 total = lane64(upto, kWave - 1);
+    const u64 upto = L::scan(sum), total = L::total(sum);
     const double target = s.target(total);
-    const u64 found = __ballot(static_cast<double>(upto) > target);
-    if (lane != __ffsll(found) - 1) return;
+    // the first lane that passes it is the one whose lanes before do not
+    if (!(static_cast<double>(upto) > target) || static_cast<double>(upto - sum) > target) return;
     u64 run = upto - sum;
     int at = -1;
     float chosen = m;
@@ -322,6 +394,14 @@ constexpr float kBinsPerUnit = 32.0f;  // linear bins of 1/32 of (max - z) / T: 
 constexpr int kDigit = 10;             // bits of a digit: a bin each
 static_assert(kBins == 1 << kDigit, "a bin for each digit");
 constexpr int kCandidates = 1024;
+
+struct Ones {
+    template <int N>
+    __device__ __forceinline__ void operator()(const float (&)[N], u64 (&w)[N]) const {
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = 1;
+    }
+};
 
 struct Shared {
     u64 bins[kBins];
@@ -393,13 +473,15 @@ struct Sampler {
     template <typename F, typename B>
     __device__ __forceinline__ bool cut_at(F f, B border_of, unsigned floor, unsigned& key, u64& above) {
         clear_bins();
-        row.each([&](const float (&v)[V], int) {
+        const float under = floor ? from_ordered(floor) : -INFINITY;
+        row.each_with([&](float top) { return top > under; },
+                      [&](const float (&v)[V], int) {
+                          u64 w[V];
+                          f(v, w);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if (masked(v[e]) || ordered(v[e]) <= floor) continue;
-                atomicAdd(&s.bins[bin_of(v[e])], f(v[e]));
-            }
-        });
+                          for (int e = 0; e < V; ++e)
+                              if (v[e] > under) atomicAdd(&s.bins[bin_of(v[e])], w[e]);
+                      });
         __syncthreads();
         if (t < kWave) {
             u64 all = 0;
@@ -422,10 +504,9 @@ struct Sampler {
         row.each([&](const float (&v)[V], int) {
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const unsigned k = ordered(v[e]);
-                if (masked(v[e]) || k <= floor || bin_of(v[e]) != bin) continue;
-                low = min(low, k);
-                high = max(high, k);
+                if (!(v[e] > under) || bin_of(v[e]) != bin) continue;
+                low = min(low, ordered(v[e]));
+                high = max(high, ordered(v[e]));
             }
         });
         if (low <= high) {
@@ -435,6 +516,7 @@ struct Sampler {
         __syncthreads();
         low = s.low;
         high = s.high;
+        const float least = from_ordered(low), most = from_ordered(high);
         unsigned prefix = low;  // the keys still searched agree with it above `bits`
         int bits = low == high ? 0 : 32 - __clz(low ^ high);
         while (bits > 0) {
@@ -444,10 +526,13 @@ struct Sampler {
             row.each([&](const float (&v)[V], int) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
+                    if (!(v[e] >= least) || !(v[e] <= most)) continue;
                     const unsigned k = ordered(v[e]);
-                    if (k < low || k > high || masked(v[e])) continue;
                     if (bits < 32 && ((k ^ prefix) >> bits)) continue;
-                    atomicAdd(&s.bins[kBins - 1 - ((k >> shift) & ((1u << digit) - 1))], f(v[e]));
+                    const float one[1] = {v[e]};
+                    u64 w[1];
+                    f(one, w);
+                    atomicAdd(&s.bins[kBins - 1 - ((k >> shift) & ((1u << digit) - 1))], w[0]);
                 }
             });
             __syncthreads();
@@ -624,8 +709,7 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
             ties = s.count;
         } else {
             if (top_k) __syncthreads();
-            if (top_k && sampler.cut_at([](float) { return 1ULL; }, [&](u64) { return static_cast<double>(set.top_k); }, 0u,
-                                        cut, above)) {
+            if (top_k && sampler.cut_at(Ones(), [&](u64) { return static_cast<double>(set.top_k); }, 0u, cut, above)) {
                 key = cut;
                 ties = set.top_k - static_cast<int>(above);
             }
@@ -634,8 +718,7 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
                 const bool limited = ties != INT_MAX;
                 u64 tie = limited ? weight(from_ordered(key)) : 0;
                 const u64 tied_mass = limited ? tie * static_cast<u64>(ties) : 0;
-                const bool found = sampler.cut_at([&](float z) { return weight(z); },
-                                                  [&](u64 all) { return set.top_p * static_cast<double>(all + tied_mass); },
+                const bool found = sampler.cut_at(weight, [&](u64 all) { return set.top_p * static_cast<double>(all + tied_mass); },
                                                   limited ? key : 0u, cut, above);
                 if (found) {
                     key = cut;
@@ -651,24 +734,26 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
     if (tie < set.min_weight) tie = 0;
 
     // kept mass (without ties) and ties of every segment of 64 chunks, in index order
-    const auto kept = [&](float z) -> u64 {
-        const u64 w = weight(z);
-        return (ties == INT_MAX ? z >= least : z > least) && w >= set.min_weight ? w : 0;
+    const bool cuts = ties != INT_MAX;
+    const auto kept = [&](const float (&v)[V], u64 (&w)[V]) {
+        weight(v, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) w[e] = w[e] < set.min_weight || (cuts && !(v[e] > least)) ? 0 : w[e];
     };
-    const auto is_tie = [&](float z) { return ties != INT_MAX && z == least; };
     const int segments = row.passes() * G::kWaves;
     row.each_pass([&](int i, const float (&v)[V], float top) {
         u64 sum = 0;
         int equal = 0;
         if (__ballot(top >= least)) {
+            u64 w[V];
+            kept(v, w);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                if (__ballot(v[e] >= least) == 0) continue;
-                sum += kept(v[e]);
-                equal += is_tie(v[e]);
+                sum += w[e];
+                equal += cuts && v[e] == least;
             }
             sum = wave_total(sum);
-            if (ties != INT_MAX) equal = wave_total(equal);
+            if (cuts) equal = wave_total(equal);
         }
         if (lane == 0) {
             mass[i * G::kWaves + G::wave()] = sum;
@@ -719,12 +804,13 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
     T::unpack(row.read(chunk), v);
     int equal = 0;
 #pragma unroll
-    for (int e = 0; e < V; ++e) equal += is_tie(v[e]);
+    for (int e = 0; e < V; ++e) equal += cuts && v[e] == least;
     int rank = tied[segment] + wave_scan(equal) - equal;
     u64 w[V], sum = 0;
+    kept(v, w);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        w[e] = is_tie(v[e]) ? (rank++ < ties ? tie : 0) : kept(v[e]);
+        if (cuts && v[e] == least) w[e] = rank++ < ties ? tie : 0;
         sum += w[e];
     }
     const u64 upto = before + wave_scan(sum);
@@ -744,9 +830,10 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
     drawn(p, r, at, chosen, m, set.per_t, total);
 }
 
-template <typename T, int E>
-void launch_wave(const Params& p, hipStream_t stream) {
-    hipLaunchKernelGGL((sample_wave<T, E>), dim3(ceil_div(p.rows, kRowsPerBlock)), dim3(kRowsPerBlock * kWave), 0, stream, p);
+template <typename T, int Lanes, int E>
+void launch_short(const Params& p, hipStream_t stream) {
+    hipLaunchKernelGGL((sample_short<T, Lanes, E>), dim3(ceil_div(p.rows, kShortThreads / Lanes)), dim3(kShortThreads), 0,
+                       stream, p);
 }
 
 template <typename T, int Group, bool Held>
@@ -759,11 +846,12 @@ void launch_block(const Params& p, hipStream_t stream) {
 template <typename T>
 void launch(const Params& p, hipStream_t stream) {
     constexpr int kHeld = tokens::kHeldChunks * T::kPerChunk;  // classes a thread can hold
-    if (p.classes <= 64) launch_wave<T, 1>(p, stream);
-    else if (p.classes <= 128) launch_wave<T, 2>(p, stream);
-    else if (p.classes <= 256) launch_wave<T, 4>(p, stream);
-    else if (p.classes <= 512) launch_wave<T, 8>(p, stream);
-    else if (p.classes <= 1024) launch_wave<T, 16>(p, stream);
+    if (p.classes <= 32) launch_short<T, 16, 2>(p, stream);
+    else if (p.classes <= 64) launch_short<T, 16, 4>(p, stream);
+    else if (p.classes <= 128) launch_short<T, 16, 8>(p, stream);
+    else if (p.classes <= 256) launch_short<T, 16, 16>(p, stream);
+    else if (p.classes <= 512) launch_short<T, 64, 8>(p, stream);
+    else if (p.classes <= 1024) launch_short<T, 64, 16>(p, stream);
     else if (p.classes <= 256 * kHeld && (p.rows > 512 || p.classes <= 4096)) launch_block<T, 256, true>(p, stream);
     else if (p.classes <= 1024 * kHeld) launch_block<T, 1024, true>(p, stream);
     else launch_block<T, 1024, false>(p, stream);

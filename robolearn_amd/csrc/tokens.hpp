@@ -16,6 +16,7 @@ struct F32 {
     typedef float Store;
     static constexpr int kPerChunk = 4;
     static constexpr unsigned kNegInf = 0xff800000u;  // -infinity in every element of a 32-bit word
+    static constexpr int kKeyShift = 0;  // last bits in which the values, as fp32, cannot differ
     __device__ __forceinline__ static void unpack(const uint4& c, float (&v)[4]) {
         v[0] = __uint_as_float(c.x), v[1] = __uint_as_float(c.y);
         v[2] = __uint_as_float(c.z), v[3] = __uint_as_float(c.w);
@@ -31,6 +32,7 @@ struct Bf16 {
     typedef unsigned short Store;
     static constexpr int kPerChunk = 8;
     static constexpr unsigned kNegInf = 0xff80ff80u;
+    static constexpr int kKeyShift = 16;
     __device__ __forceinline__ static void unpack(const uint4& c, float (&v)[8]) {
         const unsigned w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
@@ -51,6 +53,7 @@ struct F16 {
     typedef unsigned short Store;
     static constexpr int kPerChunk = 8;
     static constexpr unsigned kNegInf = 0xfc00fc00u;
+    static constexpr int kKeyShift = 13;
     __device__ __forceinline__ static void unpack(const uint4& c, float (&v)[8]) {
         const unsigned w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
