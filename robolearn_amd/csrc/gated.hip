@@ -18,26 +18,53 @@
 #include <cmath>
 #include <type_traits>
 
+RL_API std::size_t rl_gemm_workspace(int mode, int m, int n, int k, int batch, int splits) noexcept;
+
 namespace rl {
 namespace gated {
 
 enum Activation : int { kSilu = 0, kGelu = 1, kRelu = 2 };
 
-// act(g) and act'(g).
-__device__ __forceinline__ void activate(float g, int kind, float& value, float& slope) {
-    if (kind == kRelu) {
+// act(g) and act'(g).  The reciprocals and powers of two are the hardware's (1 ulp).  gelu: with E = exp(-g^2 / 2), which
+// the slope needs anyway, Phi(-|g|) = E P(1 / (1 + 0.4 |g| / sqrt 2)), P a polynomial of degree 8 fitted to
+// erfcx(x) / 2 over 0 <= x <= 10 by iteratively weighted least squares: 4.3e-7 relative in fp32, tails included.
+template <int Kind>
+__device__ __forceinline__ void activate(float g, float& value, float& slope) {
+    constexpr float kLog2e = 1.44269504088896340736f;
+    if constexpr (Kind == kRelu) {
         value = g > 0.0f ? g : 0.0f;
         slope = g > 0.0f ? 1.0f : 0.0f;
-    } else if (kind == kSilu) {
-        const float s = 1.0f / (1.0f + __expf(-g));
+    } else if constexpr (Kind == kSilu) {
+        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * g));
         value = g * s;
         slope = s * (1.0f + g * (1.0f - s));
     } else {
-        const float phi = 0.5f * erfcf(-0.70710678118654752440f * g);
+        const float e = __builtin_amdgcn_exp2f((-0.5f * kLog2e) * (g * g));
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.28284271247461900976f, fabsf(g), 1.0f));
+        float q = 0.03533526510000229f;
+        q = __builtin_fmaf(q, t, -0.1904902458190918f);
+        q = __builtin_fmaf(q, t, 0.3330724537372589f);
+        q = __builtin_fmaf(q, t, -0.18317051231861115f);
+        q = __builtin_fmaf(q, t, 0.2072092741727829f);
+        q = __builtin_fmaf(q, t, 0.06584122031927109f);
+        q = __builtin_fmaf(q, t, 0.12010600417852402f);
+        q = __builtin_fmaf(q, t, 0.1120610386133194f);
+        q = __builtin_fmaf(q, t, 3.543297134456225e-05f) * e;
+        const float phi = g >= 0.0f ? 1.0f - q : q;
         value = g * phi;
-        slope = phi + g * (0.39894228040143267794f * __expf(-0.5f * g * g));
+        slope = __builtin_fmaf(g, 0.39894228040143267794f * e, phi);
     }
 }
+
+// f(std::integral_constant<int, kind>) for the activation that runs.
+template <typename F>
+void with_activation(int kind, F f) {
+    if (kind == kSilu) f(std::integral_constant<int, kSilu>{});
+    else if (kind == kGelu) f(std::integral_constant<int, kGelu>{});
+    else f(std::integral_constant<int, kRelu>{});
+}
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // The 16-bit operand types.
 struct Bf16 {
@@ -45,6 +72,9 @@ struct Bf16 {
     typedef __bf16 Fragment __attribute__((ext_vector_type(8)));
     __device__ __forceinline__ static gemm::f32x16_t mfma(Fragment a, Fragment b, gemm::f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+    __device__ __forceinline__ static f32x4 mfma16(Fragment a, Fragment b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
     __device__ __forceinline__ static unsigned short rounded(float v) { return f32_to_bf16_bits(v); }
     __device__ __forceinline__ static float value(unsigned short b) { return bf16_bits_to_f32(b); }
@@ -54,6 +84,9 @@ struct F16 {
     typedef _Float16 Fragment __attribute__((ext_vector_type(8)));
     __device__ __forceinline__ static gemm::f32x16_t mfma(Fragment a, Fragment b, gemm::f32x16_t c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+    __device__ __forceinline__ static f32x4 mfma16(Fragment a, Fragment b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
     __device__ __forceinline__ static unsigned short rounded(float v) { return f32_to_f16_bits(v); }
     __device__ __forceinline__ static float value(unsigned short b) {
@@ -85,10 +118,17 @@ struct Product {
     long long ld_h;
     unsigned short* dpre;        // backward: [m][2 pitch], the gate's half first; columns n .. pitch are zeroed
     long long pitch;
-    int activation;
+    // plain: output rows fold .. m are the rows fold_to .. of the output, rows fold_to .. fold none (dW: the gate's rows up
+    // to a multiple of 8, then the up projection's)
+    int fold, fold_to;
 };
 
 enum Epilogue : int { kPlain = 0, kForward = 1, kBackward = 2 };
+
+// The output row of row r, -1 for none.
+__device__ __forceinline__ long long folded(int r, int fold, int fold_to) {
+    return r >= fold ? r - fold + fold_to : r < fold_to ? r : -1;
+}
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4), may_alias));
 
@@ -100,8 +140,11 @@ constexpr long long kMaxPitch = 1LL << 21;
 // LDS slot of 16-byte chunk c of row r (K-contiguous stage, 128-byte rows): the 16 rows of one ds_read_b128 phase
 // lie in 16 distinct bank groups.
 __device__ __forceinline__ int chunk_slot(int r, int c) { return c ^ ((r >> 1) & 7); }
-// The same for granule c of K row k of an M/N-contiguous stage, read transposed.
-__device__ __forceinline__ int granule_slot(int k, int c) { return c ^ (4 * (k & 3)); }
+// The same for granule c of K row k of an M/N-contiguous stage of `Rows` values a K row, read transposed.
+template <int Rows>
+__device__ __forceinline__ int granule_slot(int k, int c) {
+    return c ^ (4 * (k & 3) & (Rows / 8 - 1));
+}
 
 // Copies one K tile of an operand (Rows x kDepth) into LDS by DMA, 1 KiB an instruction.
 template <bool MN, int Rows, int Waves>
@@ -119,7 +162,7 @@ struct Loader {
             if constexpr (MN) {
                 constexpr int kGranules = Rows / 8;
                 const int k = q * (64 / kGranules) + lane / kGranules;
-                offset[j] = static_cast<unsigned>((k * ld + granule_slot(k, lane % kGranules) * 8) * 2);
+                offset[j] = static_cast<unsigned>((k * ld + granule_slot<Rows>(k, lane % kGranules) * 8) * 2);
                 chunk[j] = 0;
             } else {
                 const int row = q * 8 + lane / 8;
@@ -160,32 +203,44 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// A wave's fragments of one operand: N blocks of 32 rows from row `first` of a stage (a multiple of 32), 16 K values a step.
 template <typename T, bool MN, int Rows, int N>
-__device__ __forceinline__ void fragments(const unsigned short* stage, int first, int s, int lane,
-                                          typename T::Fragment (&f)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
+struct Reader {
+    int at[MN ? N : kDepth / 16];  // element offsets: the lane's of each block (MN), or of each step
+
+    __device__ __forceinline__ void init(int first, int lane) {
         if constexpr (MN) {
-            // the transposing read gives lane l of 16 the M offset l and four K rows: lane l addresses K row l / 4
-            // of them, M offset 4 (l % 4)
-            typedef short s16x4 __attribute__((ext_vector_type(4)));
-            s16x4 part[2];
+            // the transposing read gives lane l of 16 the M offset l and four K rows: lane l addresses K row l / 4 of
+            // them, M offset 4 (l % 4); a step's K rows differ from step 0's by multiples of 4, so their slots agree
+            const int k = 8 * (lane / 32) + (lane % 16) / 4;
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int k = 16 * s + 8 * (lane / 32) + 4 * r + (lane % 16) / 4;
+            for (int i = 0; i < N; ++i) {
                 const int granule = (first + 32 * i) / 8 + 2 * ((lane / 16) % 2) + (lane % 4) / 2;
-                const unsigned short* p = stage + k * Rows + granule_slot(k, granule) * 8 + 4 * (lane % 2);
-                part[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+                at[i] = k * Rows + granule_slot<Rows>(k, granule) * 8 + 4 * (lane % 2);
             }
-            f[i] = __builtin_bit_cast(typename T::Fragment,
-                                      __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            const int row = first + 32 * i + lane % 32;
-            f[i] = *reinterpret_cast<const typename T::Fragment*>(stage + row * kDepth +
-                                                                   chunk_slot(row, 2 * s + lane / 32) * 8);
+            // blocks lie 32 rows apart, which leaves a chunk's slot as it is
+            const int row = first + lane % 32;
+#pragma unroll
+            for (int s = 0; s < kDepth / 16; ++s) at[s] = row * kDepth + chunk_slot(lane % 32, 2 * s + lane / 32) * 8;
         }
     }
-}
+    __device__ __forceinline__ void read(const unsigned short* stage, int s, typename T::Fragment (&f)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (MN) {
+                typedef short s16x4 __attribute__((ext_vector_type(4)));
+                const unsigned short* p = stage + at[i] + 16 * s * Rows;
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+                const s16x4 hi =
+                    __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p + 4 * Rows));
+                f[i] = __builtin_bit_cast(typename T::Fragment, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            } else {
+                f[i] = *reinterpret_cast<const typename T::Fragment*>(stage + at[s] + 32 * i * kDepth);
+            }
+        }
+    }
+};
 
 // Workgroup b of the launch -> tile: consecutive tiles share operand panels, and each XCD (workgroups go to the 8 of
 // them in turn) takes a contiguous run of tiles, walked in groups of 4 M tiles.
@@ -204,7 +259,7 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& tm, int& 
     tn = local / group;
 }
 
-template <typename T, bool AMN, bool BMN, int TM, int TN, int WavesM, int WavesN, int Out>
+template <typename T, bool AMN, bool BMN, int TM, int TN, int WavesM, int WavesN, int Out, int Kind>
 __global__ __launch_bounds__(WavesM * WavesN * kWave, 1) void product_kernel(Product p, int tiles_m, int tiles_n) {
     constexpr int kWaves = WavesM * WavesN;
     constexpr int kThreadCount = kWaves * kWave;
@@ -254,36 +309,59 @@ __global__ __launch_bounds__(WavesM * WavesN * kWave, 1) void product_kernel(Pro
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
 
-    const auto multiply = [&](const unsigned short* stage) {
-#pragma unroll
-        for (int s = 0; s < kDepth / 16; ++s) {
-            typename T::Fragment a[MI], b[NJ];
-            fragments<T, AMN, TM, MI>(stage, wm * (TM / WavesM), s, lane, a);
-            fragments<T, BMN, TN, NJ>(stage + TM * kDepth, wn * (TN / WavesN), s, lane, b);
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) acc[i][j] = T::mfma(a[i], b[j], acc[i][j]);
-        }
+    Reader<T, AMN, TM, MI> ra;
+    Reader<T, BMN, TN, NJ> rb;
+    ra.init(wm * (TM / WavesM), lane);
+    rb.init(wn * (TN / WavesN), lane);
+    // One K tile from `stage`.  Fragments of the next 16-deep step are read under this step's products, those of the next
+    // K tile (in `other`) under the last one's: before it every wave's DMA of that tile has landed and every wave holds
+    // its last fragments of this one, so that `stage` takes the K tile after the next.
+    typename T::Fragment fa[2][MI], fb[2][NJ];
+    const auto read = [&](const unsigned short* stage, int s, int slot) {
+        ra.read(stage, s, fa[slot]);
+        rb.read(stage + TM * kDepth, s, fb[slot]);
     };
-
-    if (first_tile < last_tile) fetch(stage0);
-    for (int kt = first_tile; kt < last_tile; kt += 2) {
-        stage_barrier();
-        if (kt + 1 < last_tile) fetch(stage1);
-        multiply(stage0);
-        if (kt + 1 >= last_tile) break;
-        stage_barrier();
-        if (kt + 2 < last_tile) fetch(stage0);
-        multiply(stage1);
+    const auto multiply = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) acc[i][j] = T::mfma(fa[slot][i], fb[slot][j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int tiles = last_tile - first_tile;
+    const auto k_tile = [&](int kt, unsigned short* stage, const unsigned short* other) {
+        constexpr int kSteps = kDepth / 16;
+        static_assert(kSteps % 2 == 0, "a K tile ends with the second fragments");
+#pragma unroll
+        for (int s = 0; s + 1 < kSteps; ++s) {
+            read(stage, s + 1, (s + 1) % 2);
+            multiply(s % 2);
+        }
+        if (kt + 1 < tiles) {
+            stage_barrier();
+            if (kt + 2 < tiles) fetch(stage);
+            read(other, 0, 0);
+        }
+        multiply((kSteps - 1) % 2);
+    };
+    fetch(stage0);
+    stage_barrier();
+    if (tiles > 1) fetch(stage1);
+    read(stage0, 0, 0);
+    int kt = 0;
+    for (; kt + 1 < tiles; kt += 2) {
+        k_tile(kt, stage0, stage1);
+        k_tile(kt + 1, stage1, stage0);
     }
+    if (kt < tiles) k_tile(kt, stage0, stage1);
 
     // accumulator element v of lane l: column l % 32, row 8 (v / 4) + 4 (l / 32) + v % 4 of its 32 x 32 block
     const int col = lane % 32, row4 = 4 * (lane / 32);
     if constexpr (!kGated) {
         if (p.d32) {
-            float* d = p.d32 + (p.splits > 1 ? static_cast<long long>(split) * p.m * p.n : 0);
-            const long long ldd = p.splits > 1 ? p.n : p.ldd;
+            const bool direct = p.splits == 1;
+            float* d = p.d32 + (direct ? 0 : static_cast<long long>(split) * p.m * p.n);
+            const long long ldd = direct ? p.ldd : p.n;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -293,7 +371,8 @@ __global__ __launch_bounds__(WavesM * WavesN * kWave, 1) void product_kernel(Pro
 #pragma unroll
                     for (int v = 0; v < 16; ++v) {
                         const int r = m0 + wm * (TM / WavesM) + 32 * i + 8 * (v / 4) + row4 + v % 4;
-                        if (r < p.m) d[r * ldd + c] = acc[i][j][v];
+                        const long long to = direct ? folded(r, p.fold, p.fold_to) : r;
+                        if (r < p.m && to >= 0) d[to * ldd + c] = acc[i][j][v];
                     }
                 }
             return;
@@ -305,34 +384,60 @@ __global__ __launch_bounds__(WavesM * WavesN * kWave, 1) void product_kernel(Pro
     constexpr int kPassRows = 32 * WavesM;
     static_assert(kPassRows * kPitch <= kStage, "a pass fits a stage");
     constexpr int kChunks = kOutN / 8;  // 16-byte pieces of a tile row
-    // between LDS and rows of `out` whose first `columns` values exist
-    const auto move = [&](unsigned short* lds, unsigned short* out, long long ld, int columns, int pass, auto store) {
+    // rows of `out`, whose first `columns` values exist, from LDS
+    const auto leave = [&](const unsigned short* lds, unsigned short* out, long long ld, int columns, int pass) {
         const bool wide = reinterpret_cast<std::uintptr_t>(out) % 16 == 0 && ld % 8 == 0;
         for (int q = static_cast<int>(threadIdx.x); q < kPassRows * kChunks; q += kThreadCount) {
             const int local = q / kChunks, c = n0 + q % kChunks * 8;
             const int r = m0 + local / 32 * (TM / WavesM) + 32 * pass + local % 32;
-            if (r >= p.m || c >= columns) continue;
-            unsigned short* in = lds + local * kPitch + q % kChunks * 8;
-            unsigned short* to = out + r * ld + c;
+            const long long row = kGated ? r : folded(r, p.fold, p.fold_to);
+            if (r >= p.m || row < 0 || c >= columns) continue;
+            const unsigned short* in = lds + local * kPitch + q % kChunks * 8;
+            unsigned short* to = out + row * ld + c;
             if (wide && c + 8 <= columns) {
-                u32x4& from = *reinterpret_cast<u32x4*>(in);
-                u32x4& there = *reinterpret_cast<u32x4*>(to);
-                if constexpr (decltype(store)::value) there = from;
-                else from = there;
+                *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(in);
             } else {
-                for (int e = 0; e < 8 && c + e < columns; ++e) {
-                    if constexpr (decltype(store)::value) to[e] = in[e];
-                    else in[e] = to[e];
-                }
+                for (int e = 0; e < 8 && c + e < columns; ++e) to[e] = in[e];
             }
         }
     };
+    // backward: this thread's pieces of dh, all of them before the first pass waits for one
+    constexpr int kPieces = (kPassRows * kChunks + kThreadCount - 1) / kThreadCount;
+    static_assert(kPassRows * kChunks % kThreadCount == 0, "whole pieces");
+    u32x4 dh_pieces[Out == kBackward ? MI : 1][kPieces];
+    if constexpr (Out == kBackward) {
+        const bool wide = reinterpret_cast<std::uintptr_t>(p.dh) % 16 == 0 && p.ld_dh % 8 == 0;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                const int q = static_cast<int>(threadIdx.x) + k * kThreadCount;
+                const int local = q / kChunks, c = n0 + q % kChunks * 8;
+                const int r = m0 + local / 32 * (TM / WavesM) + 32 * i + local % 32;
+                u32x4 piece{0u, 0u, 0u, 0u};
+                if (r < p.m && c < p.n) {
+                    const unsigned short* from = p.dh + r * p.ld_dh + c;
+                    if (wide && c + 8 <= p.n) {
+                        piece = *reinterpret_cast<const u32x4*>(from);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (c + e < p.n) piece[e / 2] |= static_cast<unsigned>(from[e]) << (16 * (e % 2));
+                    }
+                }
+                dh_pieces[i][k] = piece;
+            }
+    }
     unsigned short *one = stage0, *two = stage1;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         __syncthreads();  // the stages are free, and the pass before has left
         if constexpr (Out == kBackward) {
-            move(one, const_cast<unsigned short*>(p.dh), p.ld_dh, p.n, i, std::false_type{});
+#pragma unroll
+            for (int k = 0; k < kPieces; ++k) {
+                const int q = static_cast<int>(threadIdx.x) + k * kThreadCount;
+                *reinterpret_cast<u32x4*>(one + q / kChunks * kPitch + q % kChunks * 8) = dh_pieces[i][k];
+            }
             __syncthreads();
         }
 #pragma unroll
@@ -345,12 +450,11 @@ __global__ __launch_bounds__(WavesM * WavesN * kWave, 1) void product_kernel(Pro
                 lds_one += wn * 32;
                 const float up = acc[i][1][v];
                 float value, slope;
-                activate(acc[i][0][v], p.activation, value, slope);
+                activate<Kind>(acc[i][0][v], value, slope);
                 if constexpr (Out == kForward) {
                     *lds_one = T::rounded(value * up);
                 } else {
-                    // columns past the last are zero, and so is what leaves for them
-                    const float dh = n0 + wn * 32 + col < p.n ? T::value(*lds_one) : 0.0f;
+                    const float dh = T::value(*lds_one);  // 0 past the last column, and so is what leaves for it
                     *lds_one = T::rounded(dh * up * slope);
                     two[lds_one - one] = T::rounded(dh * value);
                 }
@@ -358,30 +462,173 @@ __global__ __launch_bounds__(WavesM * WavesN * kWave, 1) void product_kernel(Pro
         }
         __syncthreads();
         if constexpr (Out == kPlain) {
-            move(one, p.d, p.ldd, p.n, i, std::true_type{});
+            leave(one, p.d, p.ldd, p.n, i);
         } else if constexpr (Out == kForward) {
-            move(one, p.h, p.ld_h, p.n, i, std::true_type{});
+            leave(one, p.h, p.ld_h, p.n, i);
         } else {
-            move(one, p.dpre, 2 * p.pitch, static_cast<int>(p.pitch), i, std::true_type{});
-            move(two, p.dpre + p.pitch, 2 * p.pitch, static_cast<int>(p.pitch), i, std::true_type{});
+            leave(one, p.dpre, 2 * p.pitch, static_cast<int>(p.pitch), i);
+            leave(two, p.dpre + p.pitch, 2 * p.pitch, static_cast<int>(p.pitch), i);
         }
     }
 }
 
-template <typename T, bool AMN, bool BMN, int TM, int TN, int WavesM, int WavesN, int Out>
+template <typename T, bool AMN, bool BMN, int TM, int TN, int WavesM, int WavesN, int Out, int Kind>
 void launch_tiles(const Product& p, hipStream_t stream) {
     constexpr int kOutN = Out == kPlain ? TN : TN / 2;
     const long long tiles_m = ceil_div(p.m, TM), tiles_n = ceil_div(p.n, kOutN);
     require(tiles_m * tiles_n * p.splits <= INT_MAX, "The gated product has too many tiles.");
-    hipLaunchKernelGGL((product_kernel<T, AMN, BMN, TM, TN, WavesM, WavesN, Out>),
+    hipLaunchKernelGGL((product_kernel<T, AMN, BMN, TM, TN, WavesM, WavesN, Out, Kind>),
                        dim3(static_cast<unsigned>(tiles_m * tiles_n * p.splits)), dim3(WavesM * WavesN * kWave), 0, stream,
                        p, static_cast<int>(tiles_m), static_cast<int>(tiles_n));
     check_launch("Launch gated product");
 }
 
-template <typename T, bool AMN, bool BMN, int Out>
-void launch(const Product& p, hipStream_t stream) {
-    launch_tiles<T, AMN, BMN, 128, 128, 2, 2, Out>(p, stream);
+// The output tile and the K splits of a product.
+struct Plan {
+    int tile;  // 256, 128 or 64 rows and columns of operands
+    int splits;
+};
+
+// The fastest tile and split by what one took, alone and beside others on its CU (up to 1, 2 and 5 workgroups of
+// 256, 128 and 64 a CU).  In us per 64 of K, with r of them on each CU: 1.8; 0.5 r; 0.23 r; 0.6 at least (the loads' latency).  bf16 forward over K = 1024,
+// tiles of 256 / 128 / 64: 8192 x 4096 outputs 140 / 154 / 239 us, 1024 x 4096 31 / 22.5 / 33 us, 256 x 4096 28 / 13.5 / 12.9
+// us.  Splits of K, where the caller has a place for their sums, cost a launch and their bytes.
+Plan plan_for(long long m, long long n, long long k_tiles, int most_splits) {
+    constexpr int kCus = 256;
+    struct Tile {
+        int edge, beside;
+        double step, fixed, fixed_beside;
+    };
+    constexpr Tile kTiles[] = {{256, 1, 1.8, 5.0, 0.0}, {128, 2, 0.5, 1.5, 0.7}, {64, 5, 0.23, 1.0, 0.3}};
+    Plan best{64, 1};
+    double least = 1e30;
+    for (const Tile& tile : kTiles) {
+        for (int splits = 1; splits <= most_splits; splits *= 2) {
+            if (splits > 1 && k_tiles / splits < 4) break;
+            const long long tiles = static_cast<long long>(ceil_div(m, tile.edge)) * ceil_div(n, tile.edge) * splits;
+            const double steps = static_cast<double>(ceil_div(k_tiles, splits));
+            const auto round = [&](double r) { return r > 0 ? steps * std::max(tile.step * r, 0.6) + tile.fixed + tile.fixed_beside * r : 0.0; };
+            const long long slots = kCus * tile.beside;
+            double time = static_cast<double>(tiles / slots) * round(tile.beside) +
+                          round(static_cast<double>(ceil_div(tiles % slots, kCus)));
+            if (splits > 1) time += 4.0 + static_cast<double>(splits) * m * n * 8.0 / 4.5e6;
+            if (time < least) {
+                least = time;
+                best = {tile.edge, splits};
+            }
+        }
+    }
+    return best;
+}
+
+template <typename T, bool AMN, bool BMN, int Out, int Kind>
+void launch(const Product& p, int tile, hipStream_t stream) {
+    if (tile == 256) launch_tiles<T, AMN, BMN, 256, 256, 2, 4, Out, Kind>(p, stream);
+    else if (tile == 128) launch_tiles<T, AMN, BMN, 128, 128, 2, 2, Out, Kind>(p, stream);
+    else launch_tiles<T, AMN, BMN, 64, 64, 2, 1, Out, Kind>(p, stream);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: the weights stream through the matrix cores once
+// ---------------------------------------------------------------------------
+// A workgroup makes 16 hidden values of up to 16 Tiles rows of x: its 4 waves take turns over K, 64 values a step, whose
+// pieces each lane loads straight into the fragments of v_mfma_f32_16x16x32 (lane l: weight row, or row of x, l % 16,
+// and K 16 (l / 16) .. + 15 of the step, so that a row's 128 bytes are read by two instructions), and the waves' sums
+// meet in LDS.  No staging: all loads of four steps are in flight at once.  Rows of any alignment.
+constexpr int kStreamRows = 64;  // most rows
+
+struct __attribute__((packed, aligned(2))) Piece {
+    unsigned w[4];
+};
+
+// Eight values of a row from k on, zeros past the row's end.
+template <typename T>
+__device__ __forceinline__ typename T::Fragment row_piece(const unsigned short* row, int k, int columns) {
+    if (k + 8 <= columns) {
+        const Piece piece = *reinterpret_cast<const Piece*>(row + k);
+        return __builtin_bit_cast(typename T::Fragment, piece);
+    }
+    Piece piece{};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (k + e < columns) piece.w[e / 2] |= static_cast<unsigned>(row[k + e]) << (16 * (e % 2));
+    return __builtin_bit_cast(typename T::Fragment, piece);
+}
+
+template <typename T, int Tiles, int Out, int Kind>
+__global__ __launch_bounds__(256) void stream_kernel(Product p) {
+    constexpr int kWaves = 4;
+    __shared__ f32x4 sums[kWaves][Tiles][2][kWave];
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+    const int lane = static_cast<int>(threadIdx.x) % kWave;
+    const int n0 = static_cast<int>(blockIdx.x) * 16;
+    // rows past the end repeat the last: what they make is not written
+    const unsigned short* gate = p.b + min(n0 + lane % 16, p.n - 1) * p.ldb;
+    const unsigned short* up = gate + p.up;
+    const unsigned short* x[Tiles];
+#pragma unroll
+    for (int i = 0; i < Tiles; ++i) x[i] = p.a + min(16 * i + lane % 16, p.m - 1) * p.lda;
+    f32x4 acc[Tiles][2];
+#pragma unroll
+    for (int i = 0; i < Tiles; ++i) acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int k0 = 64 * wave; k0 < p.k; k0 += 64 * kWaves) {
+        const int k = k0 + 16 * (lane / 16);
+        typename T::Fragment g[2], u[2], rows[Tiles][2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            g[s] = row_piece<T>(gate, k + 8 * s, p.k);
+            u[s] = row_piece<T>(up, k + 8 * s, p.k);
+#pragma unroll
+            for (int i = 0; i < Tiles; ++i) rows[i][s] = row_piece<T>(x[i], k + 8 * s, p.k);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < Tiles; ++i) {
+                acc[i][0] = T::mfma16(g[s], rows[i][s], acc[i][0]);
+                acc[i][1] = T::mfma16(u[s], rows[i][s], acc[i][1]);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < Tiles; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) sums[wave][i][h][lane] = acc[i][h];
+    __syncthreads();
+    // wave i finishes rows 16 i ..: lane l holds row l % 16 and hidden values 4 (l / 16) .. + 3
+    const int i = wave;
+    const int r = 16 * i + lane % 16, c = n0 + 4 * (lane / 16);
+    if (i >= Tiles || r >= p.m) return;
+    f32x4 z[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        z[h] = sums[0][i][h][lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) z[h] += sums[w][i][h][lane];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float value, slope;
+        activate<Kind>(z[0][e], value, slope);
+        if constexpr (Out == kForward) {
+            if (c + e < p.n) p.h[r * p.ld_h + c + e] = T::rounded(value * z[1][e]);
+        } else {
+            if (c + e >= p.pitch) continue;
+            const bool pad = c + e >= p.n;  // zeroed
+            const float dh = pad ? 0.0f : T::value(p.dh[r * p.ld_dh + c + e]);
+            p.dpre[r * 2 * p.pitch + c + e] = pad ? 0 : T::rounded(dh * z[1][e] * slope);
+            p.dpre[r * 2 * p.pitch + p.pitch + c + e] = pad ? 0 : T::rounded(dh * value);
+        }
+    }
+}
+
+template <typename T, int Out, int Kind>
+void launch_stream(const Product& p, hipStream_t stream) {
+    const dim3 grid(ceil_div(p.n, 16)), block(256);
+    if (p.m <= 16) hipLaunchKernelGGL((stream_kernel<T, 1, Out, Kind>), grid, block, 0, stream, p);
+    else if (p.m <= 32) hipLaunchKernelGGL((stream_kernel<T, 2, Out, Kind>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((stream_kernel<T, 4, Out, Kind>), grid, block, 0, stream, p);
+    check_launch("Launch gated stream");
 }
 
 // dst[r, 0 .. pitch) = src[r, 0 .. columns), zeros after them: rows that the DMA can read in 16-byte pieces.
@@ -402,42 +649,45 @@ __global__ __launch_bounds__(256) void pack_kernel(const unsigned short* src, lo
     }
 }
 
-// fp32: gate and up [rows, hidden] of `pre` -> h
-__global__ __launch_bounds__(256) void gate_forward(const float* pre, float* h, long long ld_h, long long rows, int hidden,
-                                                    int activation) {
+// fp32: gate and up of `pre` [rows, 2 hidden] -> h
+template <int Kind>
+__global__ __launch_bounds__(256) void gate_forward(const float* pre, float* h, long long ld_h, long long rows, int hidden) {
     const long long n = rows * hidden;
     for (long long q = blockIdx.x * 256LL + threadIdx.x; q < n; q += gridDim.x * 256LL) {
+        const long long r = q / hidden, at = 2 * r * hidden + q % hidden;
         float value, slope;
-        activate(pre[q], activation, value, slope);
-        h[q / hidden * ld_h + q % hidden] = value * pre[n + q];
+        activate<Kind>(pre[at], value, slope);
+        h[r * ld_h + q % hidden] = value * pre[at + hidden];
     }
 }
 
 // fp32: gate and up of `pre` become their gradients.
+template <int Kind>
 __global__ __launch_bounds__(256) void gate_backward(float* pre, const float* dh, long long ld_dh, long long rows,
-                                                     int hidden, int activation) {
+                                                     int hidden) {
     const long long n = rows * hidden;
     for (long long q = blockIdx.x * 256LL + threadIdx.x; q < n; q += gridDim.x * 256LL) {
+        const long long r = q / hidden, at = 2 * r * hidden + q % hidden;
         float value, slope;
-        activate(pre[q], activation, value, slope);
-        const float d = dh[q / hidden * ld_dh + q % hidden];
-        const float up = pre[n + q];
-        pre[q] = d * up * slope;
-        pre[n + q] = d * value;
+        activate<Kind>(pre[at], value, slope);
+        const float d = dh[r * ld_dh + q % hidden], up = pre[at + hidden];
+        pre[at] = d * up * slope;
+        pre[at + hidden] = d * value;
     }
 }
 
 // The splits' partial products in their order.
 template <typename T>
-__global__ __launch_bounds__(256) void reduce_kernel(const float* partial, int splits, long long m, int n,
-                                                     unsigned short* d, float* d32, long long ldd) {
-    const long long total = m * n;
+__global__ __launch_bounds__(256) void reduce_kernel(const float* partial, int splits, Product p) {
+    const long long total = static_cast<long long>(p.m) * p.n;
     for (long long q = blockIdx.x * 256LL + threadIdx.x; q < total; q += gridDim.x * 256LL) {
+        const long long row = folded(static_cast<int>(q / p.n), p.fold, p.fold_to);
+        if (row < 0) continue;
         float sum = 0.0f;
         for (int s = 0; s < splits; ++s) sum += partial[s * total + q];
-        const long long at = q / n * ldd + q % n;
-        if (d32) d32[at] = sum;
-        else d[at] = T::rounded(sum);
+        const long long at = row * p.ldd + q % p.n;
+        if (p.d32) p.d32[at] = sum;
+        else p.d[at] = T::rounded(sum);
     }
 }
 
@@ -460,13 +710,10 @@ struct Sizes {
     int inputs, hidden;
 };
 
-// K splits of a product with too few tiles: at least 256 workgroups, each with 8 K tiles of 64.
-int split_tiles(long long m, long long n, long long k_tiles) {
-    const long long tiles = static_cast<long long>(ceil_div(m, 128)) * ceil_div(n, 128);
-    long long splits = 1;
-    while (tiles * splits < 256 && k_tiles / (2 * splits) >= 8 && splits < 64) splits *= 2;
-    return static_cast<int>(splits);
-}
+constexpr int kMostSplits = 64;
+
+Plan dx_plan(const Sizes& s) { return plan_for(s.rows, s.inputs, 2LL * ceil_div(s.hidden, kDepth), kMostSplits); }
+Plan dw_plan(const Sizes& s) { return plan_for(2 * align8(s.hidden), s.inputs, ceil_div(s.rows, kDepth), kMostSplits); }
 
 struct Layout {
     std::size_t x, w, dpre, partial, bytes;
@@ -487,31 +734,46 @@ Layout layout_of(const Sizes& s, bool backward) {
     l.w = take(2LL * s.hidden * pitch, 2);
     if (backward) {
         l.dpre = take(s.rows * 2 * hidden_pitch, 2);
-        const int dx_splits = split_tiles(s.rows, s.inputs, 2 * ceil_div(s.hidden, kDepth));
-        const int dw_splits = split_tiles(s.hidden, s.inputs, ceil_div(s.rows, kDepth));
+        const int dx_splits = dx_plan(s).splits, dw_splits = dw_plan(s).splits;
         const long long dx = dx_splits > 1 ? dx_splits * s.rows * s.inputs : 0;
-        const long long dw = dw_splits > 1 ? dw_splits * static_cast<long long>(s.hidden) * s.inputs : 0;
+        const long long dw = dw_splits > 1 ? dw_splits * 2 * hidden_pitch * s.inputs : 0;
         l.partial = take(std::max(dx, dw), 4);
     }
     l.bytes = at;
     return l;
 }
 
-// K splits of the fp32 weight gradient: as the framework splits its own.
-int fp32_splits(long long m, long long n, long long k) {
-    const long long tiles = static_cast<long long>(ceil_div(m, 128)) * ceil_div(n, 128) * 2;
+// K splits of the fp32 products, as the framework splits its own: the input gradient's to 1024 tiles of 64 x 64, 256 of K
+// each; the weight gradient's to 512 of 128 x 128, 384 of K each, where that makes 256 of them.
+int fp32_dx_splits(const Sizes& s) {
+    const long long tiles = static_cast<long long>(ceil_div(s.rows, 64)) * ceil_div(s.inputs, 64), k = 2LL * s.hidden;
     int splits = 1;
-    while (tiles * splits < 512 && splits * 2 <= k / 384 && splits < 64) splits *= 2;
+    while (tiles * splits < 1024 && k / (2 * splits) >= 256 && splits < 16) splits *= 2;
+    return splits;
+}
+int fp32_dw_splits(const Sizes& s) {
+    const long long m = 2LL * s.hidden, n = s.inputs;
+    int splits = 1;
+    if (m > 64 && n > 64) {
+        const long long wide = static_cast<long long>(ceil_div(m, 128)) * ceil_div(n, 128);
+        while (wide * splits < 512 && splits * 2 <= s.rows / 384 && splits < 256) splits *= 2;
+        if (wide * splits >= 256) return splits;
+        splits = 1;
+    }
+    const long long tiles = static_cast<long long>(ceil_div(m, 64)) * ceil_div(n, 64), steps = (s.rows + 15) / 16;
+    while (tiles * splits < 1024 && splits * 2 <= std::max<long long>(1, steps / (m * n <= 65536 ? 4 : 16)) && splits < 256)
+        splits *= 2;
     return splits;
 }
 
+std::size_t fp32_partial_bytes(const Sizes& s) {
+    const std::size_t dx = rl_gemm_workspace(2, static_cast<int>(s.rows), s.inputs, 2 * s.hidden, 1, fp32_dx_splits(s));
+    const std::size_t dw = rl_gemm_workspace(2, 2 * s.hidden, s.inputs, static_cast<int>(s.rows), 1, fp32_dw_splits(s));
+    return std::max(dx, dw);
+}
+
 std::size_t fp32_bytes(const Sizes& s, bool backward) {
-    std::size_t bytes = aligned_bytes(static_cast<std::size_t>(2 * s.rows * s.hidden) * 4);
-    if (backward) {
-        const int splits = fp32_splits(s.hidden, s.inputs, s.rows);
-        if (splits > 1) bytes += aligned_bytes(static_cast<std::size_t>(splits) * 2 * s.hidden * s.inputs * 4);
-    }
-    return bytes;
+    return aligned_bytes(static_cast<std::size_t>(2 * s.rows * s.hidden) * 4) + (backward ? fp32_partial_bytes(s) : 0);
 }
 
 std::size_t workspace_bytes(const Sizes& s, bool backward) {
@@ -527,52 +789,54 @@ struct Operands {
 };
 
 void run_fp32(const Sizes& s, const Operands& o, bool backward, hipStream_t stream) {
-    const int rows = static_cast<int>(s.rows), in = s.inputs, hidden = s.hidden;
+    const int rows = static_cast<int>(s.rows), in = s.inputs, both = 2 * s.hidden;
     const float *x = static_cast<const float*>(o.x), *w = static_cast<const float*>(o.w);
-    float* pre = reinterpret_cast<float*>(o.workspace);
-    const long long each = s.rows * hidden, weights = static_cast<long long>(hidden) * in;
-    run_gemm(2, 0, 0, 1, 1, rows, hidden, in, 2, x, o.ldx, 0, w, in, weights, nullptr, pre, hidden, each, nullptr, 0, 0.0f,
-             0, 1, nullptr, 0, stream, nullptr, nullptr, nullptr);
+    float* pre = reinterpret_cast<float*>(o.workspace);  // [rows, 2 hidden]: gate, up
+    const long long each = s.rows * s.hidden;
+    run_gemm(2, 0, 0, 1, 1, rows, both, in, 1, x, o.ldx, 0, w, in, 0, nullptr, pre, both, 0, nullptr, 0, 0.0f, 0, 1, nullptr, 0,
+             stream, nullptr, nullptr, nullptr);
     if (!backward) {
-        hipLaunchKernelGGL(gate_forward, dim3(blocks_for(each)), dim3(256), 0, stream, pre, static_cast<float*>(o.h), o.ld_h,
-                           s.rows, hidden, o.activation);
+        with_activation(o.activation, [&](auto kind) {
+            hipLaunchKernelGGL((gate_forward<decltype(kind)::value>), dim3(blocks_for(each)), dim3(256), 0, stream, pre,
+                               static_cast<float*>(o.h), o.ld_h, s.rows, s.hidden);
+        });
         check_launch("Launch gating");
         return;
     }
-    hipLaunchKernelGGL(gate_backward, dim3(blocks_for(each)), dim3(256), 0, stream, pre, static_cast<const float*>(o.dh),
-                       o.ld_dh, s.rows, hidden, o.activation);
+    with_activation(o.activation, [&](auto kind) {
+        hipLaunchKernelGGL((gate_backward<decltype(kind)::value>), dim3(blocks_for(each)), dim3(256), 0, stream, pre,
+                           static_cast<const float*>(o.dh), o.ld_dh, s.rows, s.hidden);
+    });
     check_launch("Launch gating gradient");
+    float* partial = reinterpret_cast<float*>(o.workspace + aligned_bytes(static_cast<std::size_t>(2 * each) * 4));
+    const std::size_t bytes = fp32_partial_bytes(s);
     if (o.dx) {
-        float* dx = static_cast<float*>(o.dx);
-        for (int half = 0; half < 2; ++half)
-            run_gemm(2, 0, 0, 1, 0, rows, in, hidden, 1, pre + half * each, hidden, 0, w + half * weights, in, 0,
-                     half ? dx : nullptr, dx, o.ld_dx, 0, nullptr, 0, half ? 1.0f : 0.0f, 0, 1, nullptr, 0, stream, nullptr,
-                     nullptr, nullptr);
+        const int splits = fp32_dx_splits(s);
+        run_gemm(2, 0, 0, 1, 0, rows, in, both, 1, pre, both, 0, w, in, 0, nullptr, static_cast<float*>(o.dx), o.ld_dx, 0,
+                 nullptr, 0, 0.0f, 0, splits, splits > 1 ? partial : nullptr, bytes, stream, nullptr, nullptr, nullptr);
     }
     if (o.dw) {
-        const int splits = fp32_splits(hidden, in, s.rows);
-        char* partial = o.workspace + aligned_bytes(static_cast<std::size_t>(2 * each) * 4);
-        run_gemm(2, 0, 0, 0, 0, hidden, in, rows, 2, pre, hidden, each, x, o.ldx, 0, nullptr, static_cast<float*>(o.dw), in,
-                 weights, nullptr, 0, 0.0f, 0, splits, splits > 1 ? reinterpret_cast<float*>(partial) : nullptr,
-                 splits > 1 ? static_cast<std::size_t>(splits) * 2 * weights * 4 : 0, stream, nullptr, nullptr, nullptr);
+        const int splits = fp32_dw_splits(s);
+        run_gemm(2, 0, 0, 0, 0, both, in, rows, 1, pre, both, 0, x, o.ldx, 0, nullptr, static_cast<float*>(o.dw), in, 0,
+                 nullptr, 0, 0.0f, 0, splits, splits > 1 ? partial : nullptr, bytes, stream, nullptr, nullptr, nullptr);
     }
 }
 
 template <typename T, bool AMN, bool BMN>
-void run_plain(Product p, int splits, float* partial, hipStream_t stream) {
+void run_plain(Product p, const Plan& plan, float* partial, hipStream_t stream) {
     const int tiles = static_cast<int>(ceil_div(p.k, kDepth)) * p.segments;
-    p.tiles_per_split = static_cast<int>(ceil_div(tiles, splits));
+    p.tiles_per_split = static_cast<int>(ceil_div(tiles, plan.splits));
     p.splits = static_cast<int>(ceil_div(tiles, p.tiles_per_split));
     if (p.splits <= 1) {
-        launch<T, AMN, BMN, kPlain>(p, stream);
+        launch<T, AMN, BMN, kPlain, kRelu>(p, plan.tile, stream);
         return;
     }
     Product parts = p;
     parts.d = nullptr;
     parts.d32 = partial;
-    launch<T, AMN, BMN, kPlain>(parts, stream);
+    launch<T, AMN, BMN, kPlain, kRelu>(parts, plan.tile, stream);
     hipLaunchKernelGGL((reduce_kernel<T>), dim3(blocks_for(static_cast<long long>(p.m) * p.n)), dim3(256), 0, stream, partial,
-                       p.splits, static_cast<long long>(p.m), p.n, p.d, p.d32, p.ldd);
+                       p.splits, p);
     check_launch("Launch gated product reduction");
 }
 
@@ -596,9 +860,13 @@ const unsigned short* readable(const void* data, long long rows, int columns, lo
 template <typename T>
 void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t stream) {
     const Layout l = layout_of(s, backward);
+    const bool few = s.rows <= kStreamRows;
     long long ldx = o.ldx, ldw = s.inputs;
-    const unsigned short* x = readable(o.x, s.rows, s.inputs, ldx, o.workspace + l.x, stream);
-    const unsigned short* w = readable(o.w, 2LL * s.hidden, s.inputs, ldw, o.workspace + l.w, stream);
+    const unsigned short *x = static_cast<const unsigned short*>(o.x), *w = static_cast<const unsigned short*>(o.w);
+    if (!few || backward) {
+        x = readable(o.x, s.rows, s.inputs, ldx, o.workspace + l.x, stream);
+        w = readable(o.w, 2LL * s.hidden, s.inputs, ldw, o.workspace + l.w, stream);
+    }
     Product p{};
     p.a = x;
     p.lda = ldx;
@@ -607,15 +875,22 @@ void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t str
     p.up = s.hidden * ldw;
     p.m = static_cast<int>(s.rows);
     p.n = s.hidden;
-    p.k = static_cast<int>(align8(s.inputs));
+    p.k = few ? s.inputs : static_cast<int>(align8(s.inputs));
     p.segments = 1;
     p.splits = 1;
     p.tiles_per_split = static_cast<int>(ceil_div(p.k, kDepth));
-    p.activation = o.activation;
     p.h = static_cast<unsigned short*>(o.h);
     p.ld_h = o.ld_h;
+    const int tile = plan_for(s.rows, 2LL * s.hidden, p.tiles_per_split, 1).tile;
+    const auto project = [&](auto out) {
+        with_activation(o.activation, [&](auto kind) {
+            constexpr int kOut = decltype(out)::value, kKind = decltype(kind)::value;
+            if (few) launch_stream<T, kOut, kKind>(p, stream);
+            else launch<T, false, false, kOut, kKind>(p, tile, stream);
+        });
+    };
     if (!backward) {
-        launch<T, false, false, kForward>(p, stream);
+        project(std::integral_constant<int, kForward>{});
         return;
     }
     const long long pitch = align8(s.hidden);
@@ -625,7 +900,7 @@ void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t str
     p.ld_dh = o.ld_dh;
     p.dpre = dpre;
     p.pitch = pitch;
-    launch<T, false, false, kBackward>(p, stream);
+    project(std::integral_constant<int, kBackward>{});
     if (o.dx) {
         Product q{};
         q.a = dpre;
@@ -638,27 +913,27 @@ void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t str
         q.n = s.inputs;
         q.k = s.hidden;
         q.segments = 2;
+        q.fold = q.fold_to = INT_MAX;
         q.d = static_cast<unsigned short*>(o.dx);
         q.ldd = o.ld_dx;
-        run_plain<T, false, true>(q, split_tiles(s.rows, s.inputs, 2 * ceil_div(s.hidden, kDepth)), partial, stream);
+        run_plain<T, false, true>(q, dx_plan(s), partial, stream);
     }
     if (o.dw) {
-        for (int half = 0; half < 2; ++half) {
-            Product q{};
-            q.a = dpre + half * pitch;
-            q.lda = 2 * pitch;
-            q.b = x;
-            q.ldb = ldx;
-            q.m = s.hidden;
-            q.n = s.inputs;
-            q.k = static_cast<int>(s.rows);
-            q.segments = 1;
-            q.ldd = s.inputs;
-            const long long to = half * static_cast<long long>(s.hidden) * s.inputs;
-            if (o.dw_fp32) q.d32 = static_cast<float*>(o.dw) + to;
-            else q.d = static_cast<unsigned short*>(o.dw) + to;
-            run_plain<T, true, true>(q, split_tiles(s.hidden, s.inputs, ceil_div(s.rows, kDepth)), partial, stream);
-        }
+        Product q{};
+        q.a = dpre;
+        q.lda = 2 * pitch;
+        q.b = x;
+        q.ldb = ldx;
+        q.m = static_cast<int>(2 * pitch);
+        q.n = s.inputs;
+        q.k = static_cast<int>(s.rows);
+        q.segments = 1;
+        q.ldd = s.inputs;
+        q.fold = static_cast<int>(pitch);
+        q.fold_to = s.hidden;
+        if (o.dw_fp32) q.d32 = static_cast<float*>(o.dw);
+        else q.d = static_cast<unsigned short*>(o.dw);
+        run_plain<T, true, true>(q, dw_plan(s), partial, stream);
     }
 }
 
@@ -667,9 +942,9 @@ void check_sizes(const Sizes& s) {
     require(s.rows >= 0 && s.rows <= (1 << 24) && s.inputs > 0 && s.hidden > 0 && s.inputs <= (1 << 20) &&
                 s.hidden <= (1 << 20),
             "Gated products take 0 to 2^24 rows and 1 to 2^20 inputs and hidden values.");
-    require(static_cast<long long>(s.inputs) * s.hidden <= INT_MAX && s.rows * s.hidden <= INT_MAX &&
+    require(2LL * s.inputs * s.hidden <= INT_MAX && 2 * s.rows * s.hidden <= INT_MAX &&
                 s.rows * s.inputs <= INT_MAX,
-            "A gated product's matrices hold at most 2^31 - 1 values each.");
+            "A gated product's matrices (both halves of them) hold at most 2^31 - 1 values each.");
 }
 
 void run(const Sizes& s, const Operands& o, std::size_t bytes, bool backward, hipStream_t stream) {

@@ -427,7 +427,7 @@ def _type(tensor, name):
 
 
 def _current(*tensors):
-    """All on the current device, on whose current stream the call is enqueued."""
+    """The current device's current stream; every tensor has to be on that device."""
     device = None
     for tensor in tensors:
         if tensor is None:
@@ -438,6 +438,7 @@ def _current(*tensors):
             device = torch.cuda.current_device()
         if tensor.get_device() != device:
             raise ValueError(f"Every tensor must be on the current GPU (cuda:{device}), got one on {tensor.device}.")
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _matrix(tensor, shape, name, dtype=None):
@@ -489,10 +490,10 @@ def gated_forward(x, w, h, *, activation="silu", workspace=None):
     may overlap (other streams, other graphs) need one each."""
     code, rows, inputs, hidden, ldx = _gated_operands(x, w, activation)
     ld_h = _matrix(h, (rows, hidden), "h", x.dtype)
-    _current(x, w, h, workspace)
+    on = _current(x, w, h, workspace)
     _native.call("rl_gated_forward", code, rows, inputs, hidden, _ACTIVATIONS[activation], x.data_ptr(), ldx,
                  w.data_ptr(), h.data_ptr(), ld_h, ptr(workspace),
-                 0 if workspace is None else workspace.numel() * workspace.element_size(), stream())
+                 0 if workspace is None else workspace.numel() * workspace.element_size(), on)
 
 
 def gated_backward(x, w, dh, dx, dw, *, activation="silu", workspace=None):
@@ -504,11 +505,11 @@ def gated_backward(x, w, dh, dx, dw, *, activation="silu", workspace=None):
     if dw is not None and (dw.shape != w.shape or not dw.is_contiguous() or dw.dtype not in (x.dtype, torch.float32)):
         raise ValueError(f"dw must be contiguous, {list(w.shape)} and {x.dtype} or float32, got {list(dw.shape)} "
                          f"{dw.dtype}.")
-    _current(x, w, dh, dx, dw, workspace)
+    on = _current(x, w, dh, dx, dw, workspace)
     _native.call("rl_gated_backward", code, rows, inputs, hidden, _ACTIVATIONS[activation], x.data_ptr(), ldx,
                  w.data_ptr(), dh.data_ptr(), ld_dh, ptr(dx), ld_dx, ptr(dw),
                  int(dw is not None and dw.dtype == torch.float32), ptr(workspace),
-                 0 if workspace is None else workspace.numel() * workspace.element_size(), stream())
+                 0 if workspace is None else workspace.numel() * workspace.element_size(), on)
 
 
 def _distill_operands(logits, teacher_logits, teacher_index, weights, temperature):
@@ -540,10 +541,10 @@ def distill_forward(logits, teacher_logits, teacher_index, loss_rows, *, tempera
     if lse is not None:
         _vector(lse, rows, "lse")
     ldd = 0 if dlogits is None else _matrix(dlogits, (rows, classes), "dlogits", logits.dtype)
-    _current(logits, teacher_logits, teacher_index, weights, loss_rows, lse, dlogits)
+    on = _current(logits, teacher_logits, teacher_index, weights, loss_rows, lse, dlogits)
     _native.call("rl_distill_forward", logits.data_ptr(), code, ld, teacher_logits.data_ptr(), teacher,
                  teacher_index.data_ptr(), bits, ptr(weights), rows, classes, entries, float(temperature),
-                 loss_rows.data_ptr(), ptr(lse), ptr(dlogits), ldd, float(grad_scale), stream())
+                 loss_rows.data_ptr(), ptr(lse), ptr(dlogits), ldd, float(grad_scale), on)
 
 
 def distill_backward(logits, teacher_logits, teacher_index, lse, dloss_rows, dlogits, *, temperature=1.0, weights=None):
@@ -554,10 +555,10 @@ def distill_backward(logits, teacher_logits, teacher_index, lse, dloss_rows, dlo
     _vector(lse, rows, "lse")
     _vector(dloss_rows, rows, "dloss_rows")
     ldd = _matrix(dlogits, (rows, classes), "dlogits", logits.dtype)
-    _current(logits, teacher_logits, teacher_index, weights, lse, dloss_rows, dlogits)
+    on = _current(logits, teacher_logits, teacher_index, weights, lse, dloss_rows, dlogits)
     _native.call("rl_distill_backward", logits.data_ptr(), code, ld, teacher_logits.data_ptr(), teacher,
                  teacher_index.data_ptr(), bits, ptr(weights), lse.data_ptr(), dloss_rows.data_ptr(), rows, classes,
-                 entries, float(temperature), dlogits.data_ptr(), ldd, stream())
+                 entries, float(temperature), dlogits.data_ptr(), ldd, on)
 
 
 def categorical_sample(logits, uniform, tokens, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, log_probs=None):
@@ -584,6 +585,6 @@ def categorical_sample(logits, uniform, tokens, *, temperature=1.0, top_k=0, top
         else:
             scalars.append(value)
             arrays.append(None)
-    _current(logits, uniform, tokens, log_probs, *arrays)
+    on = _current(logits, uniform, tokens, log_probs, *arrays)
     _native.call("rl_categorical_sample", logits.data_ptr(), code, ld, rows, classes, *scalars, *map(ptr, arrays),
-                 uniform.data_ptr(), tokens.data_ptr(), ptr(log_probs), stream())
+                 uniform.data_ptr(), tokens.data_ptr(), ptr(log_probs), on)
