@@ -39,7 +39,8 @@ struct Params {
     void* dlogits;           // as the logits, or null
     long long ldd;
     float grad_scale;        // forward: factor of the gradient
-    double temperature;
+    double temperature, per_t;  // T, 1 / T
+    float rate;                 // log2(e) / T
     long long rows;
     int classes, entries, teacher_type, index_wide;
 };
@@ -50,6 +51,36 @@ __device__ __forceinline__ float teacher_value(const Params& p, long long at) {
     return p.teacher_type == tokens::kBf16 ? tokens::Bf16::value(bits) : tokens::F16::value(bits);
 }
 
+// LDS of a team: for every entry its logit of the teacher, its weight exp((t - max t) / T), its class and the student's
+// logit there; entries up to the next multiple of 4 are padding.
+struct Entries {
+    float *teacher, *share, *logit;
+    int* cls;
+    int padded;
+
+    __host__ __device__ static int round4(int entries) { return (entries + 3) / 4 * 4; }
+    __device__ __forceinline__ Entries(unsigned char* lds, int team, int entries) : padded(round4(entries)) {
+        teacher = reinterpret_cast<float*>(lds) + team * 4 * padded;
+        share = teacher + padded;
+        logit = share + padded;
+        cls = reinterpret_cast<int*>(logit + padded);
+    }
+    // the weights of all entries of class c
+    __device__ __forceinline__ float share_of(int c) const {
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int o = 0; o < padded; o += 4) {
+            const int4 k = *reinterpret_cast<const int4*>(cls + o);
+            const float4 e = *reinterpret_cast<const float4*>(share + o);
+            sum += k.x == c ? e.x : 0.0f;
+            sum += k.y == c ? e.y : 0.0f;
+            sum += k.z == c ? e.z : 0.0f;
+            sum += k.w == c ? e.w : 0.0f;
+        }
+        return sum;
+    }
+};
+
 template <typename T, int Group, int Held, bool Backward>
 __global__ __launch_bounds__(Group < 256 ? 256 : Group) void distill_kernel(Params p) {
     typedef typename T::Store Store;
@@ -57,59 +88,69 @@ __global__ __launch_bounds__(Group < 256 ? 256 : Group) void distill_kernel(Para
     constexpr int kTeams = Group < 256 ? 256 / Group : 1;
     constexpr int V = T::kPerChunk;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    __shared__ float scratch_all[kTeams][G::kWaves];
-    float* scratch = scratch_all[threadIdx.x / Group % kTeams];
-    // a team's entries: probability, class, and the class's logit
-    float* prob = reinterpret_cast<float*>(lds) + (threadIdx.x / Group) * 3 * p.entries;
-    int* cls = reinterpret_cast<int*>(prob + p.entries);
-    float* logit = prob + 2 * p.entries;
+    __shared__ float scratch_all[kTeams][2 * G::kWaves];
+    const int team = static_cast<int>(threadIdx.x) / Group % kTeams;
+    float* scratch = scratch_all[team];
+    const Entries entry(lds, team, p.entries);
 
-    const long long row = blockIdx.x * static_cast<long long>(kTeams) + threadIdx.x / Group;
-    if (row >= p.rows) return;  // a team of its own wave, or none of the workgroup
+    const long long row = blockIdx.x * static_cast<long long>(kTeams) + team;
+    if (row >= p.rows) return;  // a team inside a wave, or none of the workgroup
     const int t = G::thread();
     const Store* z = static_cast<const Store*>(p.logits) + row * p.ld;
     Store* dz = p.dlogits ? static_cast<Store*>(p.dlogits) + row * p.ldd : nullptr;
+    Row<T, Group, Held> r;
+    r.open(z, p.classes);
     const float weight = p.weights ? p.weights[row] : 1.0f;
+    const float rate = p.rate;
 
-    // the teacher's distribution over the row's entries
-    float top = -INFINITY;
-    bool bad = false;  // a NaN among the entries
-    for (int k = t; k < p.entries; k += Group) {
+    // the entries, and both maxima
+    float top[2] = {-INFINITY, -INFINITY};  // the teacher's, the student's
+    bool bad = false;                       // a NaN among the entries
+    for (int k = t; k < entry.padded; k += Group) {
         const long long at = row * p.entries + k;
-        const long long c = p.index_wide ? static_cast<const long long*>(p.index)[at]
-                                         : static_cast<long long>(static_cast<const int*>(p.index)[at]);
+        const bool real = k < p.entries;
+        const long long c = !real ? -1
+                            : p.index_wide ? static_cast<const long long*>(p.index)[at]
+                                           : static_cast<long long>(static_cast<const int*>(p.index)[at]);
         const bool valid = c >= 0 && c < p.classes;
         const float x = valid ? teacher_value(p, at) : -INFINITY;
-        prob[k] = x;
-        cls[k] = valid ? static_cast<int>(c) : -1;
-        logit[k] = valid ? T::value(z[c]) : -INFINITY;
-        top = fmaxf(top, x);
+        entry.teacher[k] = x;
+        entry.cls[k] = valid ? static_cast<int>(c) : -1;
+        entry.logit[k] = valid ? T::value(z[c]) : -INFINITY;
+        top[0] = fmaxf(top[0], x);
         bad |= x != x;
     }
-    if (bad) top = INFINITY;  // infinity - infinity below: the row's loss is NaN
-    top = G::max(top, scratch);
-    const float rate = static_cast<float>(kLog2e / p.temperature);
-
-    Row<T, Group, Held> r;
-    if (weight == 0.0f || top == -INFINITY) {
-        if (!Backward && t == 0) p.loss[row] = 0.0f;
-        const bool sum_wanted = !Backward && p.lse_out;
-        if (sum_wanted) {
-            r.open(z, p.classes);
-            float m = -INFINITY;
+    if (bad) top[0] = INFINITY;  // infinity - infinity below: the row's loss is NaN
+    float sums[2] = {0.0f, 1.0f};
+    if constexpr (!Backward) {
+        if constexpr (Held > 0) {
             r.each([&](int, const float (&v)[V], int) {
 #pragma unroll
-                for (int e = 0; e < V; ++e) m = fmaxf(m, v[e]);
+                for (int e = 0; e < V; ++e) top[1] = fmaxf(top[1], v[e]);
             });
-            m = G::max(m, scratch);
+        } else {
+            // one pass: a running maximum, and the sum relative to it
             float s = 0.0f;
             r.each([&](int, const float (&v)[V], int) {
+                float high = top[1];
 #pragma unroll
-                for (int e = 0; e < V; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * rate);
+                for (int e = 0; e < V; ++e) high = fmaxf(high, v[e]);
+                if (high == -INFINITY) return;
+                s *= __builtin_amdgcn_exp2f((top[1] - high) * rate);
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += __builtin_amdgcn_exp2f((v[e] - high) * rate);
+                top[1] = high;
             });
-            s = G::sum(s, scratch);
-            if (t == 0) p.lse_out[row] = static_cast<float>(m / p.temperature + log(static_cast<double>(s)));
+            sums[1] = s;
         }
+    }
+    const float mine = top[1];
+    G::max(top, scratch);
+    const float m = top[1];
+
+    const bool empty = weight == 0.0f || top[0] == -INFINITY;
+    if (empty && !(Backward ? false : p.lse_out != nullptr)) {
+        if (!Backward && t == 0) p.loss[row] = 0.0f;
         if (dz) {
             G::sync();
             for (int j = t; j < p.classes; j += Group) dz[j] = Store(0);
@@ -117,99 +158,116 @@ __global__ __launch_bounds__(Group < 256 ? 256 : Group) void distill_kernel(Para
         return;
     }
 
-    float mass = 0.0f;
-    for (int k = t; k < p.entries; k += Group) {
-        const float e = __builtin_amdgcn_exp2f((prob[k] - top) * rate);
-        mass += e;
+    // the weights of the entries and of the classes
+    for (int k = t; k < entry.padded; k += Group) {
+        const float e = empty ? 0.0f : __builtin_amdgcn_exp2f((entry.teacher[k] - top[0]) * rate);
+        entry.share[k] = e;
+        sums[0] += e;
     }
-    mass = G::sum(mass, scratch);
-
-    // the student's maximum and sum
-    r.open(z, p.classes);
-    float m = -INFINITY, s = 1.0f;
+    r.packed();
+    double log_sum = 0.0;
     if constexpr (!Backward) {
-        r.each([&](int, const float (&v)[V], int) {
+        if constexpr (Held > 0) {
+            sums[1] = 0.0f;
+            r.each([&](int, const float (&v)[V], int) {
 #pragma unroll
-            for (int e = 0; e < V; ++e) m = fmaxf(m, v[e]);
-        });
-        m = G::max(m, scratch);
-        s = 0.0f;
-        r.each([&](int, const float (&v)[V], int) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) s += __builtin_amdgcn_exp2f((v[e] - m) * rate);
-        });
-        s = G::sum(s, scratch);
+                for (int e = 0; e < V; ++e) sums[1] += __builtin_amdgcn_exp2f((v[e] - m) * rate);
+            });
+        } else if (mine != -INFINITY) {
+            sums[1] *= __builtin_amdgcn_exp2f((mine - m) * rate);
+        }
+        G::sum(sums, scratch);
+        log_sum = log(static_cast<double>(sums[1]));
+        if (t == 0 && p.lse_out) p.lse_out[row] = static_cast<float>(m * p.per_t + log_sum);
+        if (empty) {
+            if (t == 0) p.loss[row] = 0.0f;
+            if (dz) {
+                G::sync();
+                for (int j = t; j < p.classes; j += Group) dz[j] = Store(0);
+            }
+            return;
+        }
+    } else {
+        sums[0] = G::sum(sums[0], scratch);
     }
-
+    if (dz) {
+        const float factor = static_cast<float>(weight * p.temperature * (Backward ? p.dloss[row] : p.grad_scale));
+        // q(z): forward exp2((z - m) rate) / s; backward exp(z / T - lse), with 1 / T in two pieces so that the
+        // difference is rounded once
+        const float inverse = 1.0f / sums[1];
+        const float by = static_cast<float>(p.per_t);
+        const float by_rest = static_cast<float>(p.per_t - by);
+        const float lse = Backward ? p.lse_in[row] : 0.0f;
+        const auto q = [&](float x) {
+            if constexpr (Backward) {
+                x = fmaxf(x, -FLT_MAX);  // -infinity times a negative rest would be infinity
+                return __builtin_amdgcn_exp2f((__builtin_fmaf(x, by, -lse) + x * by_rest) * kLog2e);
+            } else {
+                return __builtin_amdgcn_exp2f((x - m) * rate) * inverse;
+            }
+        };
+        G::sync();  // every logit of the entries is read: the gradient may take the logits' place
+        r.packed();
+        r.each([&](int, const float (&v)[V], int first) {
+            if (first >= p.classes) return;
+            float d[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] = factor * q(v[e]);
+            if (first + V <= p.classes) {
+                const uint4 c = T::pack(d);
+                *reinterpret_cast<tokens::Chunk<Store>*>(dz + first) = {{c.x, c.y, c.z, c.w}};
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (first + e < p.classes) dz[first + e] = T::rounded(d[e]);
+            }
+        });
+        G::sync();  // the classes of the entries are written again below
+        for (int k = t; k < p.entries; k += Group) {
+            const int c = entry.cls[k];
+            if (c >= 0) dz[c] = T::rounded(factor * (q(entry.logit[k]) - entry.share_of(c) / sums[0]));
+        }
+    }
     if constexpr (!Backward) {
-        const double log_sum = log(static_cast<double>(s)), log_mass = log(static_cast<double>(mass));
+        // last, under the gradient's stores
+        const double log_mass = log(static_cast<double>(sums[0]));
         double terms = 0.0;
         for (int k = t; k < p.entries; k += Group) {
-            const float e = __builtin_amdgcn_exp2f((prob[k] - top) * rate);
+            const float e = entry.share[k];
             if (e == 0.0f) continue;
-            const double log_p = (static_cast<double>(prob[k]) - top) / p.temperature - log_mass;
-            const double log_q = (static_cast<double>(logit[k]) - m) / p.temperature - log_sum;
+            const double log_p = (static_cast<double>(entry.teacher[k]) - top[0]) * p.per_t - log_mass;
+            const double log_q = (static_cast<double>(entry.logit[k]) - m) * p.per_t - log_sum;
             terms += e * (log_p - log_q);
         }
-        // fp32 holds the sum: its terms are rounded once
-        const float total = G::sum(static_cast<float>(terms / mass), scratch);
-        if (t == 0) {
-            p.loss[row] = static_cast<float>(weight * p.temperature * p.temperature * total);
-            if (p.lse_out) p.lse_out[row] = static_cast<float>(m / p.temperature + log_sum);
-        }
+        const float total = G::sum(static_cast<float>(terms), scratch);
+        if (t == 0) p.loss[row] = static_cast<float>(weight * p.temperature * p.temperature * (total / sums[0]));
     }
-    if (!dz) return;
+}
 
-    const float factor = static_cast<float>(weight * p.temperature * (Backward ? p.dloss[row] : p.grad_scale));
-    // q(z): forward exp2((z - m) rate) / s; backward exp(z / T - lse), with 1 / T in two pieces so that the
-    // difference is rounded once
-    const float inverse = 1.0f / s;
-    const float by = static_cast<float>(1.0 / p.temperature);
-    const float by_rest = static_cast<float>(1.0 / p.temperature - by);
-    const float lse = Backward ? p.lse_in[row] : 0.0f;
-    const auto q = [&](float x) {
-        if constexpr (Backward) {
-            x = fmaxf(x, -FLT_MAX);  // -infinity times a negative rest would be infinity
-            return __builtin_amdgcn_exp2f((__builtin_fmaf(x, by, -lse) + x * by_rest) * kLog2e);
-        } else {
-            return __builtin_amdgcn_exp2f((x - m) * rate) * inverse;
-        }
-    };
-    G::sync();  // every logit of the entries is read: the gradient may take the logits' place
-    r.each([&](int, const float (&v)[V], int first) {
-        if (first >= p.classes) return;
-        float d[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) d[e] = factor * q(v[e]);
-        if (first + V <= p.classes) {
-            const uint4 c = T::pack(d);
-            *reinterpret_cast<tokens::Chunk<Store>*>(dz + first) = {{c.x, c.y, c.z, c.w}};
-        } else {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                if (first + e < p.classes) dz[first + e] = T::rounded(d[e]);
-        }
-    });
-    G::sync();  // the classes of the entries are written again below
-    for (int k = t; k < p.entries; k += Group) {
-        const int c = cls[k];
-        if (c < 0) continue;
-        float sum = 0.0f;
-        for (int o = 0; o < p.entries; ++o)
-            if (cls[o] == c) sum += __builtin_amdgcn_exp2f((prob[o] - top) * rate);
-        dz[c] = T::rounded(factor * (q(logit[k]) - sum / mass));
-    }
+template <typename T, int Group, int Held, bool Backward>
+void launch_teams(const Params& p, hipStream_t stream) {
+    constexpr int kTeams = Group < 256 ? 256 / Group : 1;
+    const std::size_t lds = kTeams * 4 * sizeof(float) * static_cast<std::size_t>(Entries::round4(p.entries));
+    hipLaunchKernelGGL((distill_kernel<T, Group, Held, Backward>), dim3(ceil_div(p.rows, kTeams)),
+                       dim3(Group < 256 ? 256 : Group), lds, stream, p);
 }
 
 template <typename T, bool Backward>
 void launch(const Params& p, hipStream_t stream) {
-    const std::size_t lds = 3 * sizeof(float) * static_cast<std::size_t>(p.entries);
-    if (p.classes <= 64 * T::kPerChunk && p.entries <= 256) {
-        hipLaunchKernelGGL((distill_kernel<T, 64, 1, Backward>), dim3(ceil_div(p.rows, 4)), dim3(256), 4 * lds, stream, p);
-    } else {
-        hipLaunchKernelGGL((distill_kernel<T, 256, 0, Backward>), dim3(static_cast<unsigned>(p.rows)), dim3(256), lds,
-                           stream, p);
-    }
+    const int chunks = static_cast<int>(ceil_div(p.classes, T::kPerChunk));
+    if (chunks <= 16 && p.entries <= 64) launch_teams<T, 16, 1, Backward>(p, stream);
+    else if (chunks <= 32 && p.entries <= 64) launch_teams<T, 16, 2, Backward>(p, stream);
+    else if (chunks <= 64 && p.entries <= 256) launch_teams<T, 64, 1, Backward>(p, stream);
+    else if (chunks <= 128 && p.entries <= 256) launch_teams<T, 64, 2, Backward>(p, stream);
+    else if (chunks <= 256 && p.entries <= 256) launch_teams<T, 64, 4, Backward>(p, stream);
+    else if (chunks <= 512 && p.entries <= 256 && p.rows > 1024) launch_teams<T, 64, 8, Backward>(p, stream);
+    else if (chunks <= 256 * 2) launch_teams<T, 256, 2, Backward>(p, stream);
+    else if (chunks <= 256 * 4) launch_teams<T, 256, 4, Backward>(p, stream);
+    else if (chunks <= 256 * 8) launch_teams<T, 256, 8, Backward>(p, stream);
+    else if (chunks <= 256 * 16) launch_teams<T, 256, 16, Backward>(p, stream);
+    else if (chunks <= 1024 * 8) launch_teams<T, 1024, 8, Backward>(p, stream);
+    else if (chunks <= 1024 * 16) launch_teams<T, 1024, 16, Backward>(p, stream);
+    else launch_teams<T, 1024, 0, Backward>(p, stream);
 }
 
 void run(Params& p, int type, bool backward, hipStream_t stream) {
@@ -263,6 +321,8 @@ Params checked(const void* logits, int type, long long ld, const void* teacher, 
     p.classes = classes;
     p.entries = entries;
     p.temperature = temperature;
+    p.per_t = 1.0 / temperature;
+    p.rate = static_cast<float>(kLog2e / temperature);
     p.dlogits = const_cast<void*>(dlogits);
     p.ldd = ldd;
     return p;

@@ -79,19 +79,20 @@ struct __attribute__((packed, aligned(sizeof(Store)))) Chunk {
     unsigned w[4];
 };
 
-// A group of Group threads (a wave, or a whole workgroup) that works on one row.
+// A group of Group threads that works on one row: 16 lanes of a wave, a wave, or a whole workgroup.
 template <int Group>
 struct Team {
-    static constexpr int kWaves = Group / kWave;
-    static_assert(Group == kWave || Group % kWave == 0, "whole waves");
+    static constexpr bool kInWave = Group <= kWave;
+    static constexpr int kWaves = kInWave ? 1 : Group / kWave;
+    static_assert(Group == 16 || Group % kWave == 0, "a row of lanes or whole waves");
 
     __device__ __forceinline__ static int thread() { return static_cast<int>(threadIdx.x) % Group; }
     __device__ __forceinline__ static int wave() {
-        return Group == kWave ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+        return kInWave ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     }
     // Orders the group's memory accesses (a wave's own LDS operations execute in order).
     __device__ __forceinline__ static void sync() {
-        if constexpr (Group == kWave) {
+        if constexpr (kInWave) {
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
@@ -99,28 +100,55 @@ struct Team {
             __syncthreads();
         }
     }
-    // scratch: kWaves floats of LDS; every thread receives the result
+    // The group's sum, or maximum, of every value; every thread receives it.  scratch: N kWaves floats of LDS.
+    template <int N>
+    __device__ __forceinline__ static void sum(float (&v)[N], float* scratch) {
+        reduce(v, scratch, [](float a, float b) { return a + b; }, [](float a) { return wave_sum(a); });
+    }
+    template <int N>
+    __device__ __forceinline__ static void max(float (&v)[N], float* scratch) {
+        reduce(v, scratch, [](float a, float b) { return fmaxf(a, b); }, [](float a) { return wave_max(a); });
+    }
     __device__ __forceinline__ static float sum(float v, float* scratch) {
-        v = wave_sum(v);
-        if constexpr (Group == kWave) return v;
-        __syncthreads();
-        if (threadIdx.x % kWave == 0) scratch[wave()] = v;
-        __syncthreads();
-        float total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) total += scratch[i];
-        return total;
+        float one[1] = {v};
+        sum(one, scratch);
+        return one[0];
     }
     __device__ __forceinline__ static float max(float v, float* scratch) {
-        v = wave_max(v);
-        if constexpr (Group == kWave) return v;
-        __syncthreads();
-        if (threadIdx.x % kWave == 0) scratch[wave()] = v;
-        __syncthreads();
-        float top = scratch[0];
+        float one[1] = {v};
+        max(one, scratch);
+        return one[0];
+    }
+
+private:
+    template <int N, typename Two, typename Wave>
+    __device__ __forceinline__ static void reduce(float (&v)[N], float* scratch, Two two, Wave over_wave) {
+        if constexpr (Group == 16) {
 #pragma unroll
-        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, scratch[i]);
-        return top;
+            for (int i = 0; i < N; ++i) {
+                v[i] = two(v[i], dpp<kDppXor1>(v[i]));
+                v[i] = two(v[i], dpp<kDppXor2>(v[i]));
+                v[i] = two(v[i], dpp<kDppHalfMirror>(v[i]));
+                v[i] = two(v[i], dpp<kDppMirror>(v[i]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = over_wave(v[i]);
+            if constexpr (!kInWave) {
+                __syncthreads();
+                if (threadIdx.x % kWave == 0) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) scratch[i * kWaves + wave()] = v[i];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    v[i] = scratch[i * kWaves];
+#pragma unroll
+                    for (int w = 1; w < kWaves; ++w) v[i] = two(v[i], scratch[i * kWaves + w]);
+                }
+            }
+        }
     }
 };
 
@@ -188,6 +216,16 @@ struct Row {
         else return read(Team<Group>::thread() + i * Group);
     }
 
+    // Makes the compiler unpack the held row again after this point, instead of holding its values in two or four times as
+    // many registers.
+    __device__ __forceinline__ void packed() {
+        if constexpr (Held > 0) {
+#pragma unroll
+            for (int i = 0; i < Held; ++i)
+                asm volatile("" : "+v"(held[i].x), "+v"(held[i].y), "+v"(held[i].z), "+v"(held[i].w));
+        }
+    }
+
     // f(i, values, index of the first value) for every pass
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
@@ -201,6 +239,7 @@ struct Row {
             }
         } else {
             const int n = passes();
+#pragma unroll 4
             for (int i = 0; i < n; ++i) {
                 float v[V];
                 T::unpack(chunk(i), v);
