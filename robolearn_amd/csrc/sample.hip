@@ -394,6 +394,7 @@ constexpr float kBinsPerUnit = 32.0f;  // linear bins of 1/32 of (max - z) / T: 
 constexpr int kDigit = 10;             // bits of a digit: a bin each
 static_assert(kBins == 1 << kDigit, "a bin for each digit");
 constexpr int kCandidates = 1024;
+constexpr int kKept = 2048;
 
 struct Ones {
     template <int N>
@@ -403,16 +404,35 @@ struct Ones {
     }
 };
 
+// The borders: a count, and a share of the sum, of which the sample's sum may be off.
+struct CountBorder {
+    int k;
+    __device__ __forceinline__ double operator()(u64) const { return k; }
+    __device__ __forceinline__ double slack(u64) const { return 0.5 * k + 16; }
+};
+struct ShareBorder {
+    double share;
+    u64 tied;  // what lies below the keys looked at and still counts
+    __device__ __forceinline__ double operator()(u64 all) const { return share * static_cast<double>(all + tied); }
+    __device__ __forceinline__ double slack(u64 all) const { return 0.03 * static_cast<double>(all); }
+};
+
 struct Shared {
     u64 bins[kBins];
-    u64 list[kCandidates];  // candidates of top-k: key, then ~index
+    union {
+        u64 list[kCandidates];  // candidates of top-k: key, then ~index
+        struct {
+            float value;
+            int segment;
+        } kept[kKept];
+    };
     double table[kTable];
     u64 above;      // running sum before the bin found
     double border;
     int bin, count;
     unsigned low, high;
     float reduce[16];
-    u64 sums[16];
+    u64 sums[16], more_sums[16];
 };
 
 // Wave 0: the first bin, in order, at which the running sum reaches `border`; -1 if none does.  Leaves the sum before
@@ -438,6 +458,22 @@ __device__ __forceinline__ int find_bin(const u64* bins, u64 start, double borde
     return first * kBinsPerLane + at;
 }
 
+// The first key of [first, last] at which `reached` holds, as it does at `last` and from the first one on: 64 tries at a
+// time by a wave.
+template <typename F>
+__device__ __forceinline__ unsigned first_key(unsigned first, unsigned last, F reached) {
+    while (first < last) {
+        const unsigned step = (last - first) / kWave + 1;
+        const unsigned mine = min(first + (threadIdx.x % kWave) * step, last);
+        const u64 votes = __ballot(reached(mine));
+        const int lane = votes ? __ffsll(votes) - 1 : kWave;
+        const unsigned start = first;
+        if (lane > 0) first = min(start + (lane - 1) * step, last - 1) + 1;
+        if (lane < kWave) last = min(start + lane * step, last);
+    }
+    return last;
+}
+
 template <typename T, int Group, bool Held>
 struct Sampler {
     typedef Team<Group> G;
@@ -449,10 +485,12 @@ struct Sampler {
     const int t;
     const float m;         // the row's maximum
     const float per_bin;   // bins of a unit of logits
+    int over_count = 0;    // how many values lay above the last cut's zone
 
-    __device__ __forceinline__ int bin_of(float z) const {
-        if (z == m) return 0;
-        const float d = (m - z) * per_bin;
+    // Bins of 1 / scale from `origin` downwards; the last one takes all the rest.
+    __device__ __forceinline__ static int bin_of(float z, float origin, float scale) {
+        if (z == origin) return 0;
+        const float d = (origin - z) * scale;
         return d < kBins - 1 ? static_cast<int>(d) : kBins - 1;
     }
 
@@ -466,57 +504,145 @@ struct Sampler {
         __syncthreads();
     }
 
-    // The key, above `floor`, at which the running sum of f reaches border_of(sum of all): in `key`, with the sum of
-    // the keys above it in `above`.  False if none does; `above` is then the sum of all.  The border must be positive.
-    // A histogram over the distance to the maximum, then digits of the keys in the bin in which the border lies, from
-    // the first bit in which they differ.
-    template <typename F, typename B>
-    __device__ __forceinline__ bool cut_at(F f, B border_of, unsigned floor, unsigned& key, u64& above) {
-        clear_bins();
-        const float under = floor ? from_ordered(floor) : -INFINITY;
-        row.each_with([&](float top) { return top > under; },
-                      [&](const float (&v)[V], int) {
-                          u64 w[V];
-                          f(v, w);
+    // Sums over the workgroup, in every thread.
+    __device__ __forceinline__ void block_totals(u64& a, u64& b) {
+        a = wave_total(a);
+        b = wave_total(b);
+        if (t % kWave == 0) {
+            s.sums[t / kWave] = a;
+            s.more_sums[t / kWave] = b;
+        }
+        __syncthreads();
+        a = b = 0;
 #pragma unroll
-                          for (int e = 0; e < V; ++e)
-                              if (v[e] > under) atomicAdd(&s.bins[bin_of(v[e])], w[e]);
-                      });
+        for (int w = 0; w < G::kWaves; ++w) {
+            a += s.sums[w];
+            b += s.more_sums[w];
+        }
+    }
+
+    // Where the border probably lies, from a sample: every thread's maximum (the heavy ones are among these), and the rest
+    // of its first chunk for all its chunks.  Bins [from, to] of the distance to the maximum; false without a guess.
+    template <typename F, typename B>
+    __device__ __forceinline__ bool guess(F f, B border_of, float mine, int& from, int& to) {
+        clear_bins();
+        if (!masked(mine)) {
+            const float one[1] = {mine};
+            u64 w[1];
+            f(one, w);
+            atomicAdd(&s.bins[bin_of(mine, m, per_bin)], w[0]);
+        }
+        float v[V];
+        u64 w[V];
+        T::unpack(row.chunk(0), v);
+        f(v, w);
+        const u64 stands_for = static_cast<u64>(row.passes());
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (!masked(v[e]) && v[e] < mine) atomicAdd(&s.bins[bin_of(v[e], m, per_bin)], w[e] * stands_for);
         __syncthreads();
         if (t < kWave) {
-            u64 all = 0;
+            u64 all = 0, before;
 #pragma unroll
             for (int i = 0; i < kBinsPerLane; ++i) all += s.bins[t * kBinsPerLane + i];
-            const double border = border_of(wave_total(all));
-            u64 before;
-            const int bin = find_bin(s.bins, 0, border, before);
+            all = wave_total(all);
+            const double border = border_of(all), slack = border_of.slack(all);
+            const int first = find_bin(s.bins, 0, fmax(border - slack, 0.0), before);
+            const int last = find_bin(s.bins, 0, border + slack, before);
             if (t == 0) {
-                s.border = border;
-                s.above = before;
-                s.bin = bin;
+                s.bin = first;
+                s.count = last < 0 ? kBins - 1 : last;
             }
         }
         __syncthreads();
-        const int bin = s.bin;
-        above = s.above;
-        if (bin < 0) return false;
-        unsigned low = 0xffffffffu, high = 0;
-        row.each([&](const float (&v)[V], int) {
+        from = s.bin;
+        to = s.count;
+        return from >= 0;
+    }
+
+    // The key, above `floor`, at which the running sum of f reaches border_of(sum of all): in `key`, with the sum of
+    // the keys above it in `above`.  False if none does; `above` is then the sum of all.  The border must be positive.
+    //
+    // One pass sums f over all keys and over those above a zone, and makes a histogram of those in it; a zone that came out
+    // wrong is replaced by all keys.  Then digits of the keys in the bin in which the border lies, from the first bit in
+    // which they can differ.  An atomic for every key would cost more than its weight: 131072 bf16, top-p alone, 151 us with
+    // all keys for a zone.
+    template <typename F, typename B>
+    __device__ __forceinline__ bool cut_at(F f, B border_of, unsigned floor, float mine, unsigned& key, u64& above) {
+        over_count = 0;
+        const float under = floor ? from_ordered(floor) : -INFINITY;
+        int from = 0, to = kBins - 1;
+        if (!floor && row.passes() >= 4 && m < INFINITY && !guess(f, border_of, mine, from, to)) from = 0, to = kBins - 1;
+        float origin, bottom, scale;
+        for (;;) {
+            // the zone (bottom, origin] is what these three say, however the bins were rounded
+            origin = from > 0 ? m - from / per_bin : m;
+            bottom = to < kBins - 1 ? m - (to + 1) / per_bin : -INFINITY;
+            scale = per_bin * kBins / (to + 1 - from);
+            __syncthreads();
+            clear_bins();
+            u64 total = 0, over = 0;
+            int count = 0;
+            row.each_with([&](float top) { return top > under; },
+                          [&](const float (&v)[V], int) {
+                              u64 w[V];
+                              f(v, w);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if (!(v[e] > under) || bin_of(v[e]) != bin) continue;
-                low = min(low, ordered(v[e]));
-                high = max(high, ordered(v[e]));
+                              for (int e = 0; e < V; ++e) {
+                                  w[e] = v[e] > under ? w[e] : 0;
+                                  total += w[e];
+                                  over += v[e] > origin ? w[e] : 0;
+                                  count += __popcll(__ballot(v[e] > origin));
+                                  if (v[e] > fmaxf(bottom, under) && v[e] <= origin)
+                                      atomicAdd(&s.bins[bin_of(v[e], origin, scale)], w[e]);
+                              }
+                          });
+            if (t % kWave == 0) atomicAdd(&s.count, count);
+            block_totals(total, over);
+            over_count = s.count;
+            if (t < kWave) {
+                const double border = border_of(total);
+                u64 before = 0;
+                const int bin = static_cast<double>(over) < border ? find_bin(s.bins, over, border, before) : -1;
+                if (t == 0) {
+                    s.border = border;
+                    s.above = before;
+                    s.bin = bin;
+                }
             }
-        });
-        if (low <= high) {
-            atomicMin(&s.low, low);
-            atomicMax(&s.high, high);
+            __syncthreads();
+            above = s.above;
+            if (s.bin >= 0) break;
+            if (from == 0 && to == kBins - 1) return false;
+            from = 0, to = kBins - 1;
+        }
+        // the keys of the bin, whether they occur or not
+        unsigned low, high;
+        if (t < kWave) {
+            const int bin = s.bin;
+            const float least_of_zone = fmaxf(bottom, under);
+            const unsigned first = least_of_zone == -INFINITY ? ordered(-FLT_MAX) : ordered(least_of_zone) + 1;
+            const unsigned last = ordered(fminf(origin, m));
+            low = first_key(first, last, [&](unsigned k) { return bin_of(from_ordered(k), origin, scale) <= bin; });
+            high = bin_of(from_ordered(last), origin, scale) >= bin
+                       ? last
+                       : first_key(low, last, [&](unsigned k) { return bin_of(from_ordered(k), origin, scale) < bin; }) - 1;
+            if (t == 0) {
+                s.low = low;
+                s.high = high;
+            }
         }
         __syncthreads();
+        // of which the type holds only those whose last bits are clear (as a negative value's key: set)
+        constexpr int kShift = T::kKeyShift;
+        constexpr unsigned kRest = (1u << kShift) - 1;
         low = s.low;
         high = s.high;
+        low = low >> 31 ? (low + kRest) & ~kRest : low | kRest;
+        high = high >> 31 ? high & ~kRest : ((high + 1) & ~kRest) - 1;
         const float least = from_ordered(low), most = from_ordered(high);
+        low >>= kShift;
+        high >>= kShift;
         unsigned prefix = low;  // the keys still searched agree with it above `bits`
         int bits = low == high ? 0 : 32 - __clz(low ^ high);
         while (bits > 0) {
@@ -524,11 +650,14 @@ struct Sampler {
             __syncthreads();
             clear_bins();
             row.each([&](const float (&v)[V], int) {
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < V; ++e) any |= (v[e] >= least) & (v[e] <= most);
+                if (!any) return;
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    if (!(v[e] >= least) || !(v[e] <= most)) continue;
-                    const unsigned k = ordered(v[e]);
-                    if (bits < 32 && ((k ^ prefix) >> bits)) continue;
+                    const unsigned k = ordered(v[e]) >> kShift;
+                    if (!(v[e] >= least) || !(v[e] <= most) || (bits < 32 && ((k ^ prefix) >> bits))) continue;
                     const float one[1] = {v[e]};
                     u64 w[1];
                     f(one, w);
@@ -550,7 +679,8 @@ struct Sampler {
             prefix = (prefix & ~mask) | (value << shift);
             bits = shift;
         }
-        key = prefix;
+        key = prefix << kShift;
+        if (!(key >> 31)) key |= kRest;
         above = s.above;
         return true;
     }
@@ -560,7 +690,7 @@ struct Sampler {
     // first, and returns its length; 0 if it came out too long.
     __device__ __forceinline__ int shortlist(int k, float mine) {
         clear_bins();
-        const int bin = masked(mine) ? kBins : bin_of(mine);
+        const int bin = masked(mine) ? kBins : bin_of(mine, m, per_bin);
         if (bin < kBins) atomicAdd(&s.bins[bin], 1ULL);
         __syncthreads();
         if (t < kWave) {
@@ -709,7 +839,7 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
             ties = s.count;
         } else {
             if (top_k) __syncthreads();
-            if (top_k && sampler.cut_at(Ones(), [&](u64) { return static_cast<double>(set.top_k); }, 0u, cut, above)) {
+            if (top_k && sampler.cut_at(Ones(), CountBorder{set.top_k}, 0u, mine, cut, above)) {
                 key = cut;
                 ties = set.top_k - static_cast<int>(above);
             }
@@ -717,9 +847,8 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
                 __syncthreads();
                 const bool limited = ties != INT_MAX;
                 u64 tie = limited ? weight(from_ordered(key)) : 0;
-                const u64 tied_mass = limited ? tie * static_cast<u64>(ties) : 0;
-                const bool found = sampler.cut_at(weight, [&](u64 all) { return set.top_p * static_cast<double>(all + tied_mass); },
-                                                  limited ? key : 0u, cut, above);
+                const ShareBorder border{set.top_p, limited ? tie * static_cast<u64>(ties) : 0};
+                const bool found = sampler.cut_at(weight, border, limited ? key : 0u, mine, cut, above);
                 if (found) {
                     key = cut;
                     tie = weight(from_ordered(key));
@@ -741,25 +870,63 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
         for (int e = 0; e < V; ++e) w[e] = w[e] < set.min_weight || (cuts && !(v[e] > least)) ? 0 : w[e];
     };
     const int segments = row.passes() * G::kWaves;
-    row.each_pass([&](int i, const float (&v)[V], float top) {
-        u64 sum = 0;
-        int equal = 0;
-        if (__ballot(top >= least)) {
-            u64 w[V];
-            kept(v, w);
+    // no value below can stay: the border, and min-p's with room for its rounding
+    const float lowest = fmaxf(least, set.min_weight ? static_cast<float>(m + (log(set.min_weight / kScale) - 1e-3) / set.per_t)
+                                                     : -FLT_MAX);
+    bool summed = false;
+    if ((cuts || set.min_weight) && sampler.over_count <= kKept && lowest > -FLT_MAX && lowest < INFINITY) {
+        // where few values stay they are listed first, and only these weighed
+        __syncthreads();
+        for (int g = t; g < segments; g += Group) mass[g] = 0, tied[g] = 0;
+        if (t == 0) s.count = 0;
+        __syncthreads();
+        row.each_pass([&](int i, const float (&v)[V], float top) {
+            if (!(top >= lowest)) return;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                sum += w[e];
-                equal += cuts && v[e] == least;
+                if (!(v[e] >= lowest)) continue;
+                const int at = atomicAdd(&s.count, 1);
+                if (at < kKept) {
+                    s.kept[at].value = v[e];
+                    s.kept[at].segment = i * G::kWaves + t / kWave;
+                }
             }
-            sum = wave_total(sum);
-            if (cuts) equal = wave_total(equal);
+        });
+        __syncthreads();
+        const int count = s.count;
+        summed = count <= kKept;
+        if (summed) {
+            for (int at = t; at < count; at += Group) {
+                const float z = s.kept[at].value;
+                const int g = s.kept[at].segment;
+                const u64 w = weight(z);
+                if (cuts && z == least) atomicAdd(&tied[g], 1);
+                else if (w >= set.min_weight) atomicAdd(&mass[g], w);
+            }
         }
-        if (lane == 0) {
-            mass[i * G::kWaves + G::wave()] = sum;
-            tied[i * G::kWaves + G::wave()] = equal;
-        }
-    });
+    }
+    if (!summed) {
+        __syncthreads();
+        row.each_pass([&](int i, const float (&v)[V], float top) {
+            u64 sum = 0;
+            int equal = 0;
+            if (__ballot(top >= lowest)) {
+                u64 w[V];
+                kept(v, w);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    sum += w[e];
+                    equal += cuts && v[e] == least;
+                }
+                sum = wave_total(sum);
+                if (cuts) equal = wave_total(equal);
+            }
+            if (lane == 0) {
+                mass[i * G::kWaves + G::wave()] = sum;
+                tied[i * G::kWaves + G::wave()] = equal;
+            }
+        });
+    }
     __syncthreads();
     if (t >= kWave) return;
 
