@@ -248,8 +248,9 @@ template <typename T, int Group, int Held, bool Backward>
 void launch_teams(const Params& p, hipStream_t stream) {
     constexpr int kTeams = Group < 256 ? 256 / Group : 1;
     const std::size_t lds = kTeams * 4 * sizeof(float) * static_cast<std::size_t>(Entries::round4(p.entries));
-    hipLaunchKernelGGL((distill_kernel<T, Group, Held, Backward>), dim3(ceil_div(p.rows, kTeams)),
-                       dim3(Group < 256 ? 256 : Group), lds, stream, p);
+    constexpr int kThreads = Group < 256 ? 256 : Group;
+    hipLaunchKernelGGL((distill_kernel<T, Group, Held, Backward>), tokens::grid_for(p.rows, kTeams, kThreads), dim3(kThreads),
+                       lds, stream, p);
 }
 
 // The smallest team whose registers hold the row, 8 chunks a thread where that reaches: 4096 x 32768 bf16, loss and
@@ -295,8 +296,8 @@ Params checked(const void* logits, int type, long long ld, const void* teacher, 
     require(tokens::known_type(type) && tokens::known_type(teacher_type),
             "Distillation takes logits of type 0 (fp32), 1 (bf16) or 3 (fp16).");
     require(index_bits == 32 || index_bits == 64, "Distillation takes indices of 32 or 64 bits.");
-    require(rows >= 0 && rows <= INT_MAX && classes > 0 && classes <= (1 << 24),
-            "Distillation takes 0 to 2^31 - 1 rows of 1 to 2^24 classes.");
+    require(rows >= 0 && classes > 0 && classes <= (1 << 24),
+            "Distillation takes no negative number of rows and 1 to 2^24 classes.");
     require(entries > 0 && entries <= kMaxEntries, "Distillation takes 1 to 1024 teacher entries a row.");
     require(temperature > 0.0 && std::isfinite(temperature), "The distillation temperature must be positive and finite.");
     require(rows == 0 || (logits && teacher && index), "Distillation operands must be nonnull.");

@@ -937,6 +937,15 @@ void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t str
     }
 }
 
+struct Span {
+    const void* begin;
+    std::size_t bytes;
+    bool meets(const Span& o) const {
+        const char *a = static_cast<const char*>(begin), *b = static_cast<const char*>(o.begin);
+        return a && b && bytes && o.bytes && a < b + o.bytes && b < a + bytes;
+    }
+};
+
 void check_sizes(const Sizes& s) {
     require(s.type == 0 || s.type == 1 || s.type == 3, "Gated products take operands of type 0 (fp32), 1 (bf16) or 3 (fp16).");
     require(s.rows >= 0 && s.rows <= (1 << 24) && s.inputs > 0 && s.hidden > 0 && s.inputs <= (1 << 20) &&
@@ -960,6 +969,21 @@ void run(const Sizes& s, const Operands& o, std::size_t bytes, bool backward, hi
     require(s.rows <= 1 || (o.ldx >= s.inputs && (!o.h || o.ld_h >= s.hidden) && (!o.dh || o.ld_dh >= s.hidden) &&
                             (!o.dx || o.ld_dx >= s.inputs)),
             "The rows of a gated operand overlap.");
+    // what is written lies apart from what is read
+    const std::size_t weights = 2 * static_cast<std::size_t>(s.hidden) * s.inputs;
+    const auto bytes_of = [&](long long ld, int columns, int each) {
+        return s.rows ? (static_cast<std::size_t>(s.rows - 1) * (s.rows > 1 ? ld : 0) + columns) * each : 0;
+    };
+    const Span read[] = {{o.x, bytes_of(o.ldx, s.inputs, size)}, {o.w, weights * size}, {o.dh, bytes_of(o.ld_dh, s.hidden, size)}};
+    const Span written[] = {{o.h, bytes_of(o.ld_h, s.hidden, size)},
+                            {o.dx, bytes_of(o.ld_dx, s.inputs, size)},
+                            {o.dw, weights * (o.dw_fp32 ? 4 : size)},
+                            {o.workspace, need}};
+    for (const Span& out : written) {
+        for (const Span& in : read) require(!out.meets(in), "An output or the workspace of a gated product overlaps an input.");
+        for (const Span& other : written)
+            require(&other == &out || !out.meets(other), "Outputs and workspace of a gated product overlap.");
+    }
     if (s.rows == 0) {
         if (backward && o.dw) {  // a sum of nothing
             const long long halves = 2LL * s.hidden * s.inputs * (s.type == 0 || o.dw_fp32 ? 2 : 1);

@@ -871,7 +871,7 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
     };
     const int segments = row.passes() * G::kWaves;
     // no value below can stay: the border, and min-p's with room for its rounding
-    const float lowest = fmaxf(least, set.min_weight ? static_cast<float>(m + (log(set.min_weight / kScale) - 1e-3) / set.per_t)
+    const float lowest = fmaxf(least, set.min_weight ? __double2float_rd(m + (log(set.min_weight / kScale) - 1e-3) / set.per_t)
                                                      : -FLT_MAX);
     bool summed = false;
     if ((cuts || set.min_weight) && sampler.over_count <= kKept && lowest > -FLT_MAX && lowest < INFINITY) {
@@ -999,15 +999,14 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
 
 template <typename T, int Lanes, int E>
 void launch_short(const Params& p, hipStream_t stream) {
-    hipLaunchKernelGGL((sample_short<T, Lanes, E>), dim3(ceil_div(p.rows, kShortThreads / Lanes)), dim3(kShortThreads), 0,
-                       stream, p);
+    hipLaunchKernelGGL((sample_short<T, Lanes, E>), tokens::grid_for(p.rows, kShortThreads / Lanes, kShortThreads),
+                       dim3(kShortThreads), 0, stream, p);
 }
 
 template <typename T, int Group, bool Held>
 void launch_block(const Params& p, hipStream_t stream) {
     constexpr int kSegments = Held ? tokens::kHeldChunks * Group / kWave : kMaxClasses / (kWave * T::kPerChunk);
-    hipLaunchKernelGGL((sample_block<T, Group, Held, kSegments>), dim3(static_cast<unsigned>(p.rows)), dim3(Group), 0, stream,
-                       p);
+    hipLaunchKernelGGL((sample_block<T, Group, Held, kSegments>), tokens::grid_for(p.rows, 1, Group), dim3(Group), 0, stream, p);
 }
 
 template <typename T>
@@ -1035,8 +1034,8 @@ RL_API int rl_categorical_sample(const void* logits, int type, long long ld, lon
     return rl::guarded("rl_categorical_sample", [&] {
         using namespace rl;
         require(tokens::known_type(type), "Sampling takes logits of type 0 (fp32), 1 (bf16) or 3 (fp16).");
-        require(rows >= 0 && rows <= INT_MAX && classes > 0 && classes <= sample::kMaxClasses,
-                "Sampling takes 0 to 2^31 - 1 rows of 1 to 2^20 classes.");
+        require(rows >= 0 && classes > 0 && classes <= sample::kMaxClasses,
+                "Sampling takes no negative number of rows and 1 to 2^20 classes.");
         require(rows == 0 || (logits && uniform && tokens_out), "Sampling operands must be nonnull.");
         require(rows <= 1 || ld >= classes, "The rows of logits overlap.");
         require(aligned(logits, tokens::type_size(type)), "The logits must be aligned to their elements.");

@@ -12,6 +12,13 @@ enum Type : int { kF32 = 0, kBf16 = 1, kF16 = 3 };
 inline bool known_type(int type) { return type == kF32 || type == kBf16 || type == kF16; }
 inline int type_size(int type) { return type == kF32 ? 4 : 2; }
 
+// Workgroups of `threads` for so many rows: a launch holds fewer than 2^32 threads.
+inline dim3 grid_for(long long rows, int rows_a_group, int threads) {
+    const long long groups = (rows - 1) / rows_a_group + 1;
+    require(groups <= 0xffffffffLL / threads, "Too many rows for one launch.");
+    return dim3(static_cast<unsigned>(groups));
+}
+
 struct F32 {
     typedef float Store;
     static constexpr int kPerChunk = 4;

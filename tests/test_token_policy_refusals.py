@@ -31,7 +31,9 @@ def refused(name, arguments, match, **changes):
     (dict(hidden=0), "hidden"), (dict(inputs=1 << 17, hidden=1 << 16), "2\\^31"), (dict(activation=3), "activation"),
     (dict(activation=-1), "activation"), (dict(x=None), "nonnull"), (dict(w=None), "nonnull"), (dict(h=None), "nonnull"),
     (dict(workspace=None), "workspace"), (dict(bytes=8), "workspace"), (dict(workspace=P + 8), "workspace"),
-    (dict(ldx=15), "overlap"), (dict(ld_h=7), "overlap"), (dict(x=P + 1), "aligned"), (dict(h=P + 1), "aligned")])
+    (dict(ldx=15), "overlap"), (dict(ld_h=7), "overlap"), (dict(x=P + 1), "aligned"), (dict(h=P + 1), "aligned"),
+    (dict(h=P), "overlaps an input"), (dict(h=P + 126), "overlaps an input"), (dict(h=2 * P + 510), "overlaps an input"),
+    (dict(workspace=2 * P), "overlaps an input"), (dict(workspace=3 * P), "overlap")])
 def test_gated_forward_refuses(changes, match):
     refused("rl_gated_forward", FORWARD, match, **changes)
 
@@ -39,7 +41,8 @@ def test_gated_forward_refuses(changes, match):
 @pytest.mark.parametrize("changes,match", [
     (dict(dx=None, dw=None), "output"), (dict(dh=None), "nonnull"), (dict(ld_dh=7), "overlap"), (dict(ld_dx=15), "overlap"),
     (dict(dw=P + 1), "aligned"), (dict(dw=P + 2, dw_fp32=1), "aligned"), (dict(bytes=64), "workspace"),
-    (dict(type=0, x=P + 2), "aligned")])
+    (dict(type=0, x=P + 2), "aligned"), (dict(dx=P), "overlaps an input"), (dict(dx=3 * P), "overlaps an input"),
+    (dict(dw=2 * P), "overlaps an input"), (dict(dw=4 * P), "overlap"), (dict(workspace=5 * P), "overlap")])
 def test_gated_backward_refuses(changes, match):
     refused("rl_gated_backward", BACKWARD, match, **changes)
 
@@ -52,6 +55,7 @@ def test_gated_backward_refuses(changes, match):
     (dict(temperature=math.inf), "temperature"), (dict(temperature=math.nan), "temperature"), (dict(logits=None), "nonnull"),
     (dict(teacher=None), "nonnull"), (dict(index=None), "nonnull"), (dict(ld=99), "overlap"), (dict(ldd=99), "overlap"),
     (dict(logits=P + 1), "aligned"), (dict(index=P + 4), "aligned"), (dict(dlogits=P + 2), "place"),
+    (dict(rows=1 << 40, dlogits=1 << 60), "Too many rows"),
     (dict(dlogits=P, ldd=101), "place")])
 def test_distill_refuses(arguments, name, changes, match):
     refused(name, arguments, match, **changes)
@@ -68,7 +72,7 @@ def test_distill_refuses_missing_outputs():
 @pytest.mark.parametrize("changes,match", [
     (dict(type=2), "type"), (dict(rows=-1), "rows"), (dict(classes=0), "classes"), (dict(classes=(1 << 20) + 1), "classes"),
     (dict(logits=None), "nonnull"), (dict(uniform=None), "nonnull"), (dict(tokens=None), "nonnull"), (dict(ld=99), "overlap"),
-    (dict(logits=P + 1), "aligned"), (dict(temperature=-0.5), "temperature"), (dict(temperature=math.inf), "temperature"),
+    (dict(logits=P + 1), "aligned"), (dict(rows=1 << 40), "Too many rows"), (dict(temperature=-0.5), "temperature"), (dict(temperature=math.inf), "temperature"),
     (dict(temperature=math.nan), "temperature"), (dict(top_p=math.nan), "top_p"), (dict(min_p=math.nan), "min_p")])
 def test_sample_refuses(changes, match):
     refused("rl_categorical_sample", SAMPLE, match, **changes)
