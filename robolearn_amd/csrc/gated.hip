@@ -242,10 +242,9 @@ struct Reader {
     }
 };
 
-// Workgroup b of the launch -> tile: consecutive tiles share operand panels, and each XCD (workgroups go to the 8 of
-// them in turn) takes a contiguous run of tiles, walked in groups of 4 M tiles.
-__device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& tm, int& tn, int& split) {
-    const int total = static_cast<int>(gridDim.x), b = static_cast<int>(blockIdx.x);
+// Workgroup b of a product's `total` -> tile: consecutive tiles share operand panels, and each XCD (workgroups go to the 8
+// of them in turn) takes a contiguous run of tiles, walked in groups of 4 M tiles.
+__device__ __forceinline__ void tile_of(int b, int total, int tiles_m, int tiles_n, int& tm, int& tn, int& split) {
     const int whole = total / 8 * 8;
     const int id = b < whole ? (b % 8) * (total / 8) + b / 8 : b;
     constexpr int kGroup = 4;
@@ -259,24 +258,29 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int& tm, int& 
     tn = local / group;
 }
 
+// bf16 elements of a stage
+template <int TM, int TN>
+constexpr int stage_size() {
+    return (TM + TN) * kDepth;
+}
+
+// Tile `block` of the product's `blocks` by a workgroup of WavesM x WavesN waves.  stage0, stage1: two LDS objects of
+// stage_size (the compiler then tells reads of one from the DMA into the other).
 template <typename T, bool AMN, bool BMN, int TM, int TN, int WavesM, int WavesN, int Out, int Kind>
-__global__ __launch_bounds__(WavesM * WavesN * kWave, 1) void product_kernel(Product p, int tiles_m, int tiles_n) {
+__device__ __forceinline__ void make_tile(const Product& p, int tiles_m, int tiles_n, int block, int blocks,
+                                          unsigned short* stage0, unsigned short* stage1) {
     constexpr int kWaves = WavesM * WavesN;
     constexpr int kThreadCount = kWaves * kWave;
     constexpr int MI = TM / WavesM / 32, NJ = TN / WavesN / 32;
     constexpr bool kGated = Out != kPlain;
     static_assert(!kGated || (!AMN && !BMN && NJ == 2), "a wave's two column blocks are the gate's and the up's");
     constexpr int kOutN = kGated ? TN / 2 : TN;  // output columns of a tile
-    constexpr int kStage = (TM + TN) * kDepth;
-    // two objects: the compiler then tells reads of one stage from the DMA into the other
-    __shared__ __attribute__((aligned(1024))) unsigned short stage0[kStage];
-    __shared__ __attribute__((aligned(1024))) unsigned short stage1[kStage];
-
+    constexpr int kStage = stage_size<TM, TN>();
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
     const int lane = static_cast<int>(threadIdx.x) % kWave;
     const int wm = wave / WavesN, wn = wave % WavesN;
     int tm, tn, split;
-    tile_of(tiles_m, tiles_n, tm, tn, split);
+    tile_of(block, blocks, tiles_m, tiles_n, tm, tn, split);
     const int m0 = tm * TM, n0 = tn * kOutN;
     const int rows_a = min(TM, p.m - m0), rows_b = min(kOutN, p.n - n0);
 
@@ -472,60 +476,121 @@ __global__ __launch_bounds__(WavesM * WavesN * kWave, 1) void product_kernel(Pro
     }
 }
 
-template <typename T, bool AMN, bool BMN, int TM, int TN, int WavesM, int WavesN, int Out, int Kind>
-void launch_tiles(const Product& p, hipStream_t stream) {
-    constexpr int kOutN = Out == kPlain ? TN : TN / 2;
-    const long long tiles_m = ceil_div(p.m, TM), tiles_n = ceil_div(p.n, kOutN);
-    require(tiles_m * tiles_n * p.splits <= INT_MAX, "The gated product has too many tiles.");
-    hipLaunchKernelGGL((product_kernel<T, AMN, BMN, TM, TN, WavesM, WavesN, Out, Kind>),
-                       dim3(static_cast<unsigned>(tiles_m * tiles_n * p.splits)), dim3(WavesM * WavesN * kWave), 0, stream,
-                       p, static_cast<int>(tiles_m), static_cast<int>(tiles_n));
-    check_launch("Launch gated product");
-}
-
-// The output tile and the K splits of a product.
-struct Plan {
-    int tile;  // 256, 128 or 64 rows and columns of operands
-    int splits;
+// The waves of a tile of `Edge` rows and columns: 256 takes 2 x 4 of 128 x 64 outputs, 128 2 x 2 of 64 x 64, 64 2 x 1 of 32 x 64.
+template <int Edge>
+struct Waves {
+    static constexpr int kM = 2, kN = Edge == 256 ? 4 : Edge == 128 ? 2 : 1;
+    static constexpr int kThreads = kM * kN * kWave;
 };
 
-// The fastest tile and split by what one took, alone and beside others on its CU (up to 1, 2 and 5 workgroups of
-// 256, 128 and 64 a CU).  In us per 64 of K, with r of them on each CU: 1.8; 0.5 r; 0.23 r; 0.6 at least (the loads' latency).  bf16 forward over K = 1024,
-// tiles of 256 / 128 / 64: 8192 x 4096 outputs 140 / 154 / 239 us, 1024 x 4096 31 / 22.5 / 33 us, 256 x 4096 28 / 13.5 / 12.9
-// us.  Splits of K, where the caller has a place for their sums, cost a launch and their bytes.
-Plan plan_for(long long m, long long n, long long k_tiles, int most_splits) {
-    constexpr int kCus = 256;
-    struct Tile {
-        int edge, beside;
-        double step, fixed, fixed_beside;
-    };
-    constexpr Tile kTiles[] = {{256, 1, 1.8, 5.0, 0.0}, {128, 2, 0.5, 1.5, 0.7}, {64, 5, 0.23, 1.0, 0.3}};
-    Plan best{64, 1};
+template <typename T, int Edge, int Out, int Kind>
+__global__ __launch_bounds__(Waves<Edge>::kThreads, 1) void project_kernel(Product p, int tiles_m, int tiles_n) {
+    __shared__ __attribute__((aligned(1024))) unsigned short stage0[stage_size<Edge, Edge>()];
+    __shared__ __attribute__((aligned(1024))) unsigned short stage1[stage_size<Edge, Edge>()];
+    make_tile<T, false, false, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, Out, Kind>(
+        p, tiles_m, tiles_n, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), stage0, stage1);
+}
+
+// One of the two gradient products: its tiles, and its workgroups (0: not asked for).
+struct Share {
+    Product p;
+    int tiles_m, tiles_n, blocks;
+};
+
+// dx and dW side by side in one launch, the workgroups with more of K first: together they fill the CUs where each alone
+// would not (8192 x 1024 x 4096: 128 tiles of 256 x 256 each).
+template <typename T, int Edge>
+__global__ __launch_bounds__(Waves<Edge>::kThreads, 1) void gradients_kernel(Share dx, Share dw, int dw_first) {
+    __shared__ __attribute__((aligned(1024))) unsigned short stage0[stage_size<Edge, Edge>()];
+    __shared__ __attribute__((aligned(1024))) unsigned short stage1[stage_size<Edge, Edge>()];
+    const int block = static_cast<int>(blockIdx.x);
+    if (dw_first ? block >= dw.blocks : block < dx.blocks)
+        make_tile<T, false, true, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, kPlain, kRelu>(
+            dx.p, dx.tiles_m, dx.tiles_n, dw_first ? block - dw.blocks : block, dx.blocks, stage0, stage1);
+    else
+        make_tile<T, true, true, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, kPlain, kRelu>(
+            dw.p, dw.tiles_m, dw.tiles_n, dw_first ? block : block - dx.blocks, dw.blocks, stage0, stage1);
+}
+
+// What a tile takes: up to `beside` workgroups a CU, r of them on each; us per 64 of K and us beside that.  Measured with
+// bf16 over K = 1024 on tiles of 256 / 128 / 64: 8192 x 4096 outputs 140 / 154 / 239 us, 1024 x 4096 31 / 22.5 / 33 us, 256 x
+// 4096 28 / 13.5 / 12.9 us.
+struct TileCost {
+    int edge, beside;
+    double step, fixed, fixed_beside;
+    // 0.6 us at least a step: the loads' latency
+    double time(double steps, double r) const { return steps * std::max(step * r, 0.6) + fixed + fixed_beside * r; }
+};
+constexpr TileCost kTileCosts[] = {{256, 1, 1.8, 5.0, 0.0}, {128, 2, 0.5, 1.5, 0.7}, {64, 5, 0.23, 1.0, 0.3}};
+constexpr int kCus = 256;
+
+inline long long tiles_of(long long m, long long n, int edge) {
+    return static_cast<long long>(ceil_div(m, edge)) * ceil_div(n, edge);
+}
+
+// The tile that projects m rows onto n columns (gate and up) over k_tiles 64ths of K soonest.
+int projection_tile(long long m, long long n, long long k_tiles) {
+    int best = 64;
     double least = 1e30;
-    for (const Tile& tile : kTiles) {
-        for (int splits = 1; splits <= most_splits; splits *= 2) {
-            if (splits > 1 && k_tiles / splits < 4) break;
-            const long long tiles = static_cast<long long>(ceil_div(m, tile.edge)) * ceil_div(n, tile.edge) * splits;
-            const double steps = static_cast<double>(ceil_div(k_tiles, splits));
-            const auto round = [&](double r) { return r > 0 ? steps * std::max(tile.step * r, 0.6) + tile.fixed + tile.fixed_beside * r : 0.0; };
-            const long long slots = kCus * tile.beside;
-            double time = static_cast<double>(tiles / slots) * round(tile.beside) +
-                          round(static_cast<double>(ceil_div(tiles % slots, kCus)));
-            if (splits > 1) time += 4.0 + static_cast<double>(splits) * m * n * 8.0 / 4.5e6;
-            if (time < least) {
-                least = time;
-                best = {tile.edge, splits};
+    for (const TileCost& c : kTileCosts) {
+        const long long tiles = tiles_of(m, n, c.edge), slots = kCus * c.beside, rest = tiles % slots;
+        const double steps = static_cast<double>(k_tiles);
+        const double time = static_cast<double>(tiles / slots) * c.time(steps, c.beside) +
+                            (rest ? c.time(steps, static_cast<double>(ceil_div(rest, kCus))) : 0.0);
+        if (time < least) {
+            least = time;
+            best = c.edge;
+        }
+    }
+    return best;
+}
+
+// The tile of both gradient products and the K splits of each (whose fp32 sums cost a launch and their bytes).  It goes
+// by the sizes alone: one gradient has the same bits whether the other is asked for or not.
+struct GradientPlan {
+    int edge, dx_splits, dw_splits;
+};
+constexpr int kMostSplits = 64;
+
+GradientPlan gradient_plan(long long dx_m, long long dw_m, long long n, long long dx_tiles, long long dw_tiles) {
+    GradientPlan best{64, 1, 1};
+    double least = 1e30;
+    for (const TileCost& c : kTileCosts) {
+        const long long dx_groups = tiles_of(dx_m, n, c.edge), dw_groups = tiles_of(dw_m, n, c.edge), slots = kCus * c.beside;
+        for (int a = 1; a <= kMostSplits && (a == 1 || dx_tiles / a >= 4); a *= 2) {
+            for (int b = 1; b <= kMostSplits && (b == 1 || dw_tiles / b >= 4); b *= 2) {
+                const long long groups = dx_groups * a + dw_groups * b;
+                const double r = groups <= slots ? static_cast<double>(ceil_div(groups, kCus)) : c.beside;
+                const double dx = c.time(static_cast<double>(ceil_div(dx_tiles, a)), r);
+                const double dw = c.time(static_cast<double>(ceil_div(dw_tiles, b)), r);
+                double time = std::max(dx, dw);
+                if (groups > slots) time = 0.5 * time + (dx * dx_groups * a + dw * dw_groups * b) / slots;
+                if (a > 1 || b > 1)
+                    time += 4.0 + ((a > 1 ? a * dx_m : 0) + (b > 1 ? b * dw_m : 0)) * static_cast<double>(n) * 8.0 / 4.5e6;
+                if (time < least) {
+                    least = time;
+                    best = {c.edge, a, b};
+                }
+                if (groups > 4 * slots) break;
             }
         }
     }
     return best;
 }
 
-template <typename T, bool AMN, bool BMN, int Out, int Kind>
-void launch(const Product& p, int tile, hipStream_t stream) {
-    if (tile == 256) launch_tiles<T, AMN, BMN, 256, 256, 2, 4, Out, Kind>(p, stream);
-    else if (tile == 128) launch_tiles<T, AMN, BMN, 128, 128, 2, 2, Out, Kind>(p, stream);
-    else launch_tiles<T, AMN, BMN, 64, 64, 2, 1, Out, Kind>(p, stream);
+template <typename T, int Edge, int Out, int Kind>
+void launch_projection(const Product& p, hipStream_t stream) {
+    const long long tiles_m = ceil_div(p.m, Edge), tiles_n = ceil_div(p.n, Edge / 2);
+    hipLaunchKernelGGL((project_kernel<T, Edge, Out, Kind>), dim3(static_cast<unsigned>(tiles_m * tiles_n)),
+                       dim3(Waves<Edge>::kThreads), 0, stream, p, static_cast<int>(tiles_m), static_cast<int>(tiles_n));
+    check_launch("Launch gated projection");
+}
+
+template <typename T, int Out, int Kind>
+void launch_projection(const Product& p, int edge, hipStream_t stream) {
+    if (edge == 256) launch_projection<T, 256, Out, Kind>(p, stream);
+    else if (edge == 128) launch_projection<T, 128, Out, Kind>(p, stream);
+    else launch_projection<T, 64, Out, Kind>(p, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -631,21 +696,30 @@ void launch_stream(const Product& p, hipStream_t stream) {
     check_launch("Launch gated stream");
 }
 
-// dst[r, 0 .. pitch) = src[r, 0 .. columns), zeros after them: rows that the DMA can read in 16-byte pieces.
-__global__ __launch_bounds__(256) void pack_kernel(const unsigned short* src, long long ld, long long rows, int columns,
-                                                   unsigned short* dst, int pitch) {
-    const long long pieces = rows * (pitch / 8);
-    for (long long q = blockIdx.x * 256LL + threadIdx.x; q < pieces; q += gridDim.x * 256LL) {
-        const long long r = q / (pitch / 8);
-        const int c = static_cast<int>(q % (pitch / 8)) * 8;
+// Copies of operands whose rows the DMA cannot read in 16-byte pieces: to[r, 0 .. pitch) = from[r, 0 .. columns), then zeros.
+struct Copy {
+    const unsigned short* from;
+    unsigned short* to;
+    long long ld, rows;
+    int columns, pitch;
+    __host__ __device__ long long pieces() const { return rows * (pitch / 8); }
+};
+__global__ __launch_bounds__(256) void pack_kernel(Copy a, Copy b) {
+    const long long all = a.pieces() + b.pieces();
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
+        const bool second = i >= a.pieces();
+        const Copy& copy = second ? b : a;
+        const long long q = second ? i - a.pieces() : i;
+        const long long r = q / (copy.pitch / 8);
+        const int c = static_cast<int>(q % (copy.pitch / 8)) * 8;
+        const unsigned short* s = copy.from + r * copy.ld + c;
         unsigned w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const unsigned short* s = src + r * ld + c + 2 * e;
-            const unsigned lo = c + 2 * e < columns ? s[0] : 0u, hi = c + 2 * e + 1 < columns ? s[1] : 0u;
+            const unsigned lo = c + 2 * e < copy.columns ? s[2 * e] : 0u, hi = c + 2 * e + 1 < copy.columns ? s[2 * e + 1] : 0u;
             w[e] = lo | (hi << 16);
         }
-        *reinterpret_cast<u32x4*>(dst + r * pitch + c) = u32x4{w[0], w[1], w[2], w[3]};
+        *reinterpret_cast<u32x4*>(copy.to + r * copy.pitch + c) = u32x4{w[0], w[1], w[2], w[3]};
     }
 }
 
@@ -676,18 +750,28 @@ __global__ __launch_bounds__(256) void gate_backward(float* pre, const float* dh
     }
 }
 
-// The splits' partial products in their order.
+// Both products' splits, in their order (splits 1: nothing to add).
+struct Sum {
+    Product p;
+    const float* partial;
+    int splits;
+    __host__ __device__ long long values() const { return splits > 1 ? static_cast<long long>(p.m) * p.n : 0; }
+};
 template <typename T>
-__global__ __launch_bounds__(256) void reduce_kernel(const float* partial, int splits, Product p) {
-    const long long total = static_cast<long long>(p.m) * p.n;
-    for (long long q = blockIdx.x * 256LL + threadIdx.x; q < total; q += gridDim.x * 256LL) {
-        const long long row = folded(static_cast<int>(q / p.n), p.fold, p.fold_to);
+__global__ __launch_bounds__(256) void reduce_kernel(Sum a, Sum b) {
+    const long long all = a.values() + b.values();
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
+        const bool second = i >= a.values();
+        const Sum& s = second ? b : a;
+        const long long q = second ? i - a.values() : i, total = s.values();
+        const long long row = folded(static_cast<int>(q / s.p.n), s.p.fold, s.p.fold_to);
         if (row < 0) continue;
         float sum = 0.0f;
-        for (int s = 0; s < splits; ++s) sum += partial[s * total + q];
-        const long long at = row * p.ldd + q % p.n;
-        if (p.d32) p.d32[at] = sum;
-        else p.d[at] = T::rounded(sum);
+#pragma unroll 4
+        for (int k = 0; k < s.splits; ++k) sum += s.partial[k * total + q];
+        const long long at = row * s.p.ldd + q % s.p.n;
+        if (s.p.d32) s.p.d32[at] = sum;
+        else s.p.d[at] = T::rounded(sum);
     }
 }
 
@@ -710,13 +794,12 @@ struct Sizes {
     int inputs, hidden;
 };
 
-constexpr int kMostSplits = 64;
-
-Plan dx_plan(const Sizes& s) { return plan_for(s.rows, s.inputs, 2LL * ceil_div(s.hidden, kDepth), kMostSplits); }
-Plan dw_plan(const Sizes& s) { return plan_for(2 * align8(s.hidden), s.inputs, ceil_div(s.rows, kDepth), kMostSplits); }
+GradientPlan plan_of(const Sizes& s) {
+    return gradient_plan(s.rows, 2 * align8(s.hidden), s.inputs, 2LL * ceil_div(s.hidden, kDepth), ceil_div(s.rows, kDepth));
+}
 
 struct Layout {
-    std::size_t x, w, dpre, partial, bytes;
+    std::size_t x, w, dpre, dx_sums, dw_sums, bytes;
 };
 
 // Where the parts of a 16-bit call's workspace lie.  Copies of x and w are counted always: whether they are needed goes
@@ -734,10 +817,9 @@ Layout layout_of(const Sizes& s, bool backward) {
     l.w = take(2LL * s.hidden * pitch, 2);
     if (backward) {
         l.dpre = take(s.rows * 2 * hidden_pitch, 2);
-        const int dx_splits = dx_plan(s).splits, dw_splits = dw_plan(s).splits;
-        const long long dx = dx_splits > 1 ? dx_splits * s.rows * s.inputs : 0;
-        const long long dw = dw_splits > 1 ? dw_splits * 2 * hidden_pitch * s.inputs : 0;
-        l.partial = take(std::max(dx, dw), 4);
+        const GradientPlan plan = plan_of(s);
+        l.dx_sums = take(plan.dx_splits > 1 ? plan.dx_splits * s.rows * s.inputs : 0, 4);
+        l.dw_sums = take(plan.dw_splits > 1 ? plan.dw_splits * 2 * hidden_pitch * s.inputs : 0, 4);
     }
     l.bytes = at;
     return l;
@@ -822,39 +904,41 @@ void run_fp32(const Sizes& s, const Operands& o, bool backward, hipStream_t stre
     }
 }
 
-template <typename T, bool AMN, bool BMN>
-void run_plain(Product p, const Plan& plan, float* partial, hipStream_t stream) {
+// A gradient product's share of the launch: `splits` pieces of K, whose sums go to `sums` where they are several.
+Share share_of(const Product& p, int edge, int splits, float* sums) {
+    Share share{p, static_cast<int>(ceil_div(p.m, edge)), static_cast<int>(ceil_div(p.n, edge)), 0};
     const int tiles = static_cast<int>(ceil_div(p.k, kDepth)) * p.segments;
-    p.tiles_per_split = static_cast<int>(ceil_div(tiles, plan.splits));
-    p.splits = static_cast<int>(ceil_div(tiles, p.tiles_per_split));
-    if (p.splits <= 1) {
-        launch<T, AMN, BMN, kPlain, kRelu>(p, plan.tile, stream);
-        return;
+    share.p.tiles_per_split = static_cast<int>(ceil_div(tiles, splits));
+    share.p.splits = static_cast<int>(ceil_div(tiles, share.p.tiles_per_split));
+    const long long blocks = static_cast<long long>(share.tiles_m) * share.tiles_n * share.p.splits;
+    require(blocks <= INT_MAX / 2, "The gated product has too many tiles.");
+    share.blocks = static_cast<int>(blocks);
+    if (share.p.splits > 1) {
+        share.p.d = nullptr;
+        share.p.d32 = sums;
     }
-    Product parts = p;
-    parts.d = nullptr;
-    parts.d32 = partial;
-    launch<T, AMN, BMN, kPlain, kRelu>(parts, plan.tile, stream);
-    hipLaunchKernelGGL((reduce_kernel<T>), dim3(blocks_for(static_cast<long long>(p.m) * p.n)), dim3(256), 0, stream, partial,
-                       p.splits, p);
-    check_launch("Launch gated product reduction");
+    return share;
 }
 
-// The operand as the DMA reads it: in place, or copied to rows of 16-byte pieces.
-const unsigned short* readable(const void* data, long long rows, int columns, long long& ld, char* space,
-                               hipStream_t stream) {
+template <typename T, int Edge>
+void launch_gradients(const Share& dx, const Share& dw, hipStream_t stream) {
+    const int dw_first = dw.p.tiles_per_split > dx.p.tiles_per_split;
+    hipLaunchKernelGGL((gradients_kernel<T, Edge>), dim3(static_cast<unsigned>(dx.blocks + dw.blocks)),
+                       dim3(Waves<Edge>::kThreads), 0, stream, dx, dw, dw_first);
+    check_launch("Launch gated gradients");
+}
+
+// The operand as the DMA reads it: in place, or (`copy` filled in) in a copy with rows of 16-byte pieces.
+const unsigned short* readable(const void* data, long long rows, int columns, long long& ld, char* space, Copy& copy) {
     const unsigned short* p = static_cast<const unsigned short*>(data);
     if (aligned(p, 16) && columns % 8 == 0 && (ld % 8 == 0 || rows == 1) && ld <= kMaxPitch) {
         if (rows == 1) ld = align8(columns);
         return p;
     }
-    unsigned short* copy = reinterpret_cast<unsigned short*>(space);
-    const int pitch = static_cast<int>(align8(columns));
-    hipLaunchKernelGGL(pack_kernel, dim3(blocks_for(rows * (pitch / 8))), dim3(256), 0, stream, p, ld, rows, columns, copy,
-                       pitch);
-    check_launch("Launch operand copy");
-    ld = pitch;
-    return copy;
+    unsigned short* to = reinterpret_cast<unsigned short*>(space);
+    copy = Copy{p, to, ld, rows, columns, static_cast<int>(align8(columns))};
+    ld = copy.pitch;
+    return to;
 }
 
 template <typename T>
@@ -864,8 +948,15 @@ void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t str
     long long ldx = o.ldx, ldw = s.inputs;
     const unsigned short *x = static_cast<const unsigned short*>(o.x), *w = static_cast<const unsigned short*>(o.w);
     if (!few || backward) {
-        x = readable(o.x, s.rows, s.inputs, ldx, o.workspace + l.x, stream);
-        w = readable(o.w, 2LL * s.hidden, s.inputs, ldw, o.workspace + l.w, stream);
+        Copy copies[2]{};
+        copies[0].pitch = copies[1].pitch = 8;
+        x = readable(o.x, s.rows, s.inputs, ldx, o.workspace + l.x, copies[0]);
+        w = readable(o.w, 2LL * s.hidden, s.inputs, ldw, o.workspace + l.w, copies[1]);
+        const long long pieces = copies[0].pieces() + copies[1].pieces();
+        if (pieces > 0) {
+            hipLaunchKernelGGL(pack_kernel, dim3(blocks_for(pieces)), dim3(256), 0, stream, copies[0], copies[1]);
+            check_launch("Launch operand copies");
+        }
     }
     Product p{};
     p.a = x;
@@ -881,12 +972,12 @@ void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t str
     p.tiles_per_split = static_cast<int>(ceil_div(p.k, kDepth));
     p.h = static_cast<unsigned short*>(o.h);
     p.ld_h = o.ld_h;
-    const int tile = plan_for(s.rows, 2LL * s.hidden, p.tiles_per_split, 1).tile;
+    const int edge = projection_tile(s.rows, 2LL * s.hidden, p.tiles_per_split);
     const auto project = [&](auto out) {
         with_activation(o.activation, [&](auto kind) {
             constexpr int kOut = decltype(out)::value, kKind = decltype(kind)::value;
             if (few) launch_stream<T, kOut, kKind>(p, stream);
-            else launch<T, false, false, kOut, kKind>(p, tile, stream);
+            else launch_projection<T, kOut, kKind>(p, edge, stream);
         });
     };
     if (!backward) {
@@ -895,45 +986,49 @@ void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t str
     }
     const long long pitch = align8(s.hidden);
     unsigned short* dpre = reinterpret_cast<unsigned short*>(o.workspace + l.dpre);
-    float* partial = reinterpret_cast<float*>(o.workspace + l.partial);
     p.dh = static_cast<const unsigned short*>(o.dh);
     p.ld_dh = o.ld_dh;
     p.dpre = dpre;
     p.pitch = pitch;
     project(std::integral_constant<int, kBackward>{});
-    if (o.dx) {
-        Product q{};
-        q.a = dpre;
-        q.lda = 2 * pitch;
-        q.seg_a = pitch;
-        q.b = w;
-        q.ldb = ldw;
-        q.seg_b = s.hidden * ldw;
-        q.m = static_cast<int>(s.rows);
-        q.n = s.inputs;
-        q.k = s.hidden;
-        q.segments = 2;
-        q.fold = q.fold_to = INT_MAX;
-        q.d = static_cast<unsigned short*>(o.dx);
-        q.ldd = o.ld_dx;
-        run_plain<T, false, true>(q, dx_plan(s), partial, stream);
-    }
-    if (o.dw) {
-        Product q{};
-        q.a = dpre;
-        q.lda = 2 * pitch;
-        q.b = x;
-        q.ldb = ldx;
-        q.m = static_cast<int>(2 * pitch);
-        q.n = s.inputs;
-        q.k = static_cast<int>(s.rows);
-        q.segments = 1;
-        q.ldd = s.inputs;
-        q.fold = static_cast<int>(pitch);
-        q.fold_to = s.hidden;
-        if (o.dw_fp32) q.d32 = static_cast<float*>(o.dw);
-        else q.d = static_cast<unsigned short*>(o.dw);
-        run_plain<T, true, true>(q, dw_plan(s), partial, stream);
+
+    const GradientPlan plan = plan_of(s);
+    Product dx{}, dw{};
+    dx.a = dw.a = dpre;
+    dx.lda = dw.lda = 2 * pitch;
+    dx.n = dw.n = s.inputs;
+    dx.m = static_cast<int>(s.rows);
+    dx.k = s.hidden;
+    dx.segments = 2;
+    dx.seg_a = pitch;
+    dx.b = w;
+    dx.ldb = ldw;
+    dx.seg_b = s.hidden * ldw;
+    dx.fold = dx.fold_to = INT_MAX;
+    dx.d = static_cast<unsigned short*>(o.dx);
+    dx.ldd = o.ld_dx;
+    dw.m = static_cast<int>(2 * pitch);
+    dw.k = static_cast<int>(s.rows);
+    dw.segments = 1;
+    dw.b = x;
+    dw.ldb = ldx;
+    dw.fold = static_cast<int>(pitch);
+    dw.fold_to = s.hidden;
+    if (o.dw_fp32) dw.d32 = static_cast<float*>(o.dw);
+    else dw.d = static_cast<unsigned short*>(o.dw);
+    dw.ldd = s.inputs;
+    float *dx_sums = reinterpret_cast<float*>(o.workspace + l.dx_sums), *dw_sums = reinterpret_cast<float*>(o.workspace + l.dw_sums);
+    Share dx_share = share_of(dx, plan.edge, plan.dx_splits, dx_sums), dw_share = share_of(dw, plan.edge, plan.dw_splits, dw_sums);
+    if (!o.dx) dx_share.blocks = 0;
+    if (!o.dw) dw_share.blocks = 0;
+    if (plan.edge == 256) launch_gradients<T, 256>(dx_share, dw_share, stream);
+    else if (plan.edge == 128) launch_gradients<T, 128>(dx_share, dw_share, stream);
+    else launch_gradients<T, 64>(dx_share, dw_share, stream);
+    const Sum dx_sum{dx, dx_sums, o.dx ? dx_share.p.splits : 0}, dw_sum{dw, dw_sums, o.dw ? dw_share.p.splits : 0};
+    const long long values = dx_sum.values() + dw_sum.values();
+    if (values > 0) {
+        hipLaunchKernelGGL((reduce_kernel<T>), dim3(blocks_for(values)), dim3(256), 0, stream, dx_sum, dw_sum);
+        check_launch("Launch gated gradient sums");
     }
 }
 
