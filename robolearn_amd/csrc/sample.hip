@@ -395,6 +395,7 @@ constexpr int kDigit = 10;             // bits of a digit: a bin each
 static_assert(kBins == 1 << kDigit, "a bin for each digit");
 constexpr int kCandidates = 1024;
 constexpr int kKept = 2048;
+constexpr int kRanked = 128;      // candidates up to which counting the larger ones is faster than sorting
 
 struct Ones {
     template <int N>
@@ -420,7 +421,7 @@ struct ShareBorder {
 struct Shared {
     u64 bins[kBins];
     union {
-        u64 list[kCandidates];  // candidates of top-k: key, then ~index
+        alignas(16) u64 list[kCandidates];  // candidates of top-k: key, then ~index
         struct {
             float value;
             int segment;
@@ -716,8 +717,29 @@ struct Sampler {
         __syncthreads();
         const int count = s.count;
         if (count > min(kCandidates, Group)) return 0;
-        sort(count);
+        if (count <= kRanked) place(count);
+        else sort(count);
         return count;
+    }
+
+    // Puts each of the list's first `count` where it belongs, by how many are larger.
+    __device__ __forceinline__ void place(int count) {
+        if (t == 0) s.list[count] = 0;  // the pairs below may end with it
+        __syncthreads();
+        u64 x = 0;
+        int rank = 0;
+        if (t < count) {
+            x = s.list[t];
+            const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(s.list);
+#pragma unroll 4
+            for (int i = 0; i < (count + 1) / 2; ++i) {
+                const ulonglong2 pair = pairs[i];
+                rank += (pair.x > x) + (pair.y > x);
+            }
+        }
+        __syncthreads();
+        if (t < count) s.list[rank] = x;
+        __syncthreads();
     }
 
     // Descending bitonic sort of the list's first `count`, one a thread; partners within a wave exchange by shuffles.
@@ -766,13 +788,12 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
     __shared__ Shared s;
     __shared__ u64 mass[Segments];
     __shared__ int tied[Segments];
-    fill_table(s.table);
     const long long r = blockIdx.x;
     const int t = static_cast<int>(threadIdx.x), lane = t % kWave;
-    const Settings set(p, r);
-
     tokens::LongRow<T, Group, Held> row;
     row.open(static_cast<const Store*>(p.logits) + r * p.ld, p.classes);
+    fill_table(s.table);  // under the row's loads
+    const Settings set(p, r);
     float mine = -INFINITY;
     row.each_max([&](float top) { mine = fmaxf(mine, top); });
     const float m = G::max(mine, s.reduce);
@@ -875,25 +896,31 @@ __global__ __launch_bounds__(Group) void sample_block(Params p) {
                                                      : -FLT_MAX);
     bool summed = false;
     if ((cuts || set.min_weight) && sampler.over_count <= kKept && lowest > -FLT_MAX && lowest < INFINITY) {
-        // where few values stay they are listed first, and only these weighed
+        // where few values stay they are listed first, and only these weighed; if most threads hold one there are many
         __syncthreads();
         for (int g = t; g < segments; g += Group) mass[g] = 0, tied[g] = 0;
-        if (t == 0) s.count = 0;
+        if (t == 0) s.count = 0, s.high = 0;
         __syncthreads();
-        row.each_pass([&](int i, const float (&v)[V], float top) {
-            if (!(top >= lowest)) return;
+        const u64 holders = __ballot(mine >= lowest);
+        if (lane == 0) atomicAdd(&s.high, static_cast<unsigned>(__popcll(holders)));
+        __syncthreads();
+        int count = kKept + 1;
+        if (s.high * 8 <= Group * 7) {
+            row.each_pass([&](int i, const float (&v)[V], float top) {
+                if (!(top >= lowest)) return;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                if (!(v[e] >= lowest)) continue;
-                const int at = atomicAdd(&s.count, 1);
-                if (at < kKept) {
-                    s.kept[at].value = v[e];
-                    s.kept[at].segment = i * G::kWaves + t / kWave;
+                for (int e = 0; e < V; ++e) {
+                    if (!(v[e] >= lowest)) continue;
+                    const int at = atomicAdd(&s.count, 1);
+                    if (at < kKept) {
+                        s.kept[at].value = v[e];
+                        s.kept[at].segment = i * G::kWaves + t / kWave;
+                    }
                 }
-            }
-        });
-        __syncthreads();
-        const int count = s.count;
+            });
+            __syncthreads();
+            count = s.count;
+        }
         summed = count <= kKept;
         if (summed) {
             for (int at = t; at < count; at += Group) {
