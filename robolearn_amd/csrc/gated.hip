@@ -619,10 +619,10 @@ struct __attribute__((packed, aligned(2))) Piece {
     unsigned w[4];
 };
 
-// Eight values of a row from k on, zeros past the row's end.
-template <typename T>
+// Eight values of a row from k on; Whole: all inside the row, else zeros past its end.
+template <typename T, bool Whole>
 __device__ __forceinline__ typename T::Fragment row_piece(const unsigned short* row, int k, int columns) {
-    if (k + 8 <= columns) {
+    if (Whole || k + 8 <= columns) {
         const Piece piece = *reinterpret_cast<const Piece*>(row + k);
         return __builtin_bit_cast(typename T::Fragment, piece);
     }
@@ -649,16 +649,16 @@ __global__ __launch_bounds__(256) void stream_kernel(Product p) {
     f32x4 acc[Tiles][2];
 #pragma unroll
     for (int i = 0; i < Tiles; ++i) acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int k0 = 64 * wave; k0 < p.k; k0 += 64 * kWaves) {
+    const auto step = [&](int k0, auto whole) {
+        constexpr bool kWhole = decltype(whole)::value;
         const int k = k0 + 16 * (lane / 16);
         typename T::Fragment g[2], u[2], rows[Tiles][2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            g[s] = row_piece<T>(gate, k + 8 * s, p.k);
-            u[s] = row_piece<T>(up, k + 8 * s, p.k);
+            g[s] = row_piece<T, kWhole>(gate, k + 8 * s, p.k);
+            u[s] = row_piece<T, kWhole>(up, k + 8 * s, p.k);
 #pragma unroll
-            for (int i = 0; i < Tiles; ++i) rows[i][s] = row_piece<T>(x[i], k + 8 * s, p.k);
+            for (int i = 0; i < Tiles; ++i) rows[i][s] = row_piece<T, kWhole>(x[i], k + 8 * s, p.k);
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -667,7 +667,15 @@ __global__ __launch_bounds__(256) void stream_kernel(Product p) {
                 acc[i][0] = T::mfma16(g[s], rows[i][s], acc[i][0]);
                 acc[i][1] = T::mfma16(u[s], rows[i][s], acc[i][1]);
             }
+    };
+    int k0 = 64 * wave;
+    constexpr int kTurn = 64 * kWaves;
+    for (; k0 + 3 * kTurn + 64 <= p.k; k0 += 4 * kTurn) {
+#pragma unroll
+        for (int turn = 0; turn < 4; ++turn) step(k0 + turn * kTurn, std::true_type{});
     }
+    for (; k0 + 64 <= p.k; k0 += kTurn) step(k0, std::true_type{});
+    if (k0 < p.k) step(k0, std::false_type{});
 #pragma unroll
     for (int i = 0; i < Tiles; ++i)
 #pragma unroll
@@ -813,6 +821,7 @@ GradientPlan plan_of(const Sizes& s) {
 
 struct Layout {
     std::size_t x, w, dpre, dx_sums, dw_sums, bytes;
+    GradientPlan plan;
 };
 
 // Where the parts of a 16-bit call's workspace lie.  Copies of x and w are counted always: whether they are needed goes
@@ -830,9 +839,9 @@ Layout layout_of(const Sizes& s, bool backward) {
     l.w = take(2LL * s.hidden * pitch, 2);
     if (backward) {
         l.dpre = take(s.rows * 2 * hidden_pitch, 2);
-        const GradientPlan plan = plan_of(s);
-        l.dx_sums = take(plan.dx_splits > 1 ? plan.dx_splits * s.rows * s.inputs : 0, 4);
-        l.dw_sums = take(plan.dw_splits > 1 ? plan.dw_splits * 2 * hidden_pitch * s.inputs : 0, 4);
+        l.plan = plan_of(s);
+        l.dx_sums = take(l.plan.dx_splits > 1 ? l.plan.dx_splits * s.rows * s.inputs : 0, 4);
+        l.dw_sums = take(l.plan.dw_splits > 1 ? l.plan.dw_splits * 2 * hidden_pitch * s.inputs : 0, 4);
     }
     l.bytes = at;
     return l;
@@ -872,6 +881,7 @@ std::size_t fp32_bytes(const Sizes& s, bool backward) {
 }
 
 std::size_t workspace_bytes(const Sizes& s, bool backward) {
+    if (s.rows == 0) return 0;
     return s.type == 0 ? fp32_bytes(s, backward) : layout_of(s, backward).bytes;
 }
 
@@ -955,8 +965,7 @@ const unsigned short* readable(const void* data, long long rows, int columns, lo
 }
 
 template <typename T>
-void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t stream) {
-    const Layout l = layout_of(s, backward);
+void run_16bit(const Sizes& s, const Operands& o, const Layout& l, bool backward, hipStream_t stream) {
     const bool few = s.rows <= kStreamRows;
     long long ldx = o.ldx, ldw = s.inputs;
     const unsigned short *x = static_cast<const unsigned short*>(o.x), *w = static_cast<const unsigned short*>(o.w);
@@ -1005,7 +1014,7 @@ void run_16bit(const Sizes& s, const Operands& o, bool backward, hipStream_t str
     p.pitch = pitch;
     project(std::integral_constant<int, kBackward>{});
 
-    const GradientPlan plan = plan_of(s);
+    const GradientPlan& plan = l.plan;
     Product dx{}, dw{};
     dx.a = dw.a = dpre;
     dx.lda = dw.lda = 2 * pitch;
@@ -1067,8 +1076,10 @@ void check_sizes(const Sizes& s) {
 void run(const Sizes& s, const Operands& o, std::size_t bytes, bool backward, hipStream_t stream) {
     check_sizes(s);
     require(o.activation >= kSilu && o.activation <= kRelu, "Unknown activation: 0 silu, 1 gelu, 2 relu.");
-    const std::size_t need = workspace_bytes(s, backward);
-    require(s.rows == 0 || need == 0 || (o.workspace && bytes >= need && aligned(o.workspace, 16)),
+    Layout layout{};
+    if (s.rows > 0 && s.type != 0) layout = layout_of(s, backward);
+    const std::size_t need = s.rows == 0 ? 0 : s.type == 0 ? fp32_bytes(s, backward) : layout.bytes;
+    require(need == 0 || (o.workspace && bytes >= need && aligned(o.workspace, 16)),
             "The gated workspace is null, misaligned or too small (rl_gated_workspace).");
     const int size = s.type == 0 ? 4 : 2;
     for (const void* q : {o.x, o.w, o.dh, static_cast<const void*>(o.h), static_cast<const void*>(o.dx)})
@@ -1102,8 +1113,8 @@ void run(const Sizes& s, const Operands& o, std::size_t bytes, bool backward, hi
         return;
     }
     if (s.type == 0) run_fp32(s, o, backward, stream);
-    else if (s.type == 1) run_16bit<Bf16>(s, o, backward, stream);
-    else run_16bit<F16>(s, o, backward, stream);
+    else if (s.type == 1) run_16bit<Bf16>(s, o, layout, backward, stream);
+    else run_16bit<F16>(s, o, layout, backward, stream);
 }
 
 }  // namespace gated
@@ -1114,7 +1125,7 @@ RL_API size_t rl_gated_workspace(int type, long long rows, int inputs, int hidde
     rl::guarded("rl_gated_workspace", [&] {
         const rl::gated::Sizes s{type, rows, inputs, hidden};
         rl::gated::check_sizes(s);
-        bytes = rows ? rl::gated::workspace_bytes(s, backward != 0) : 0;
+        bytes = rl::gated::workspace_bytes(s, backward != 0);
     });
     return bytes;
 }
