@@ -118,8 +118,8 @@ struct Product {
     long long ld_h;
     unsigned short* dpre;        // backward: [m][2 pitch], the gate's half first; columns n .. pitch are zeroed
     long long pitch;
-    // plain: output rows fold .. m are the rows fold_to .. of the output, rows fold_to .. fold none (dW: the gate's rows up
-    // to a multiple of 8, then the up projection's)
+    // plain: rows 0 .. fold_to and fold .. fold + fold_to are the output's, one after the other, and the rest none (dW: the
+    // gate's rows up to a multiple of 8, then the up projection's up to one)
     int fold, fold_to;
 };
 
@@ -127,7 +127,8 @@ enum Epilogue : int { kPlain = 0, kForward = 1, kBackward = 2 };
 
 // The output row of row r, -1 for none.
 __device__ __forceinline__ long long folded(int r, int fold, int fold_to) {
-    return r >= fold ? r - fold + fold_to : r < fold_to ? r : -1;
+    const int of_half = r >= fold ? r - fold : r;
+    return of_half < fold_to ? (r >= fold ? of_half + fold_to : of_half) : -1;
 }
 
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4), may_alias));

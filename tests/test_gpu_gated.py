@@ -15,9 +15,23 @@ SHAPES = [(1, 1, 1), (1, 64, 64), (1, 1032, 520), (2, 8, 3), (5, 39, 17), (16, 1
 TYPES = [torch.bfloat16, torch.float16, torch.float32]
 
 
+BEHIND = 1 << 16  # bytes behind a buffer that a test looks at
+
+
 def workspace_for(x, w, gpu, backward):
     need = K.gated_workspace(x.shape[0], x.shape[1], w.shape[1], x.dtype, backward=backward)
-    return torch.full((max(need, 1),), 0xff, dtype=torch.uint8, device=gpu)  # NaN in every type
+    return torch.full((need + BEHIND,), 0xff, dtype=torch.uint8, device=gpu)[:need]  # NaN in every type
+
+
+def flat(shape, dtype, gpu):
+    """A contiguous tensor of sevens, and what lies behind it."""
+    values = math.prod(shape)
+    store = torch.full((values + BEHIND,), 7.0, dtype=dtype, device=gpu)
+    return store[values:], store[:values].view(shape)
+
+
+def behind(workspace):
+    return workspace.as_strided((BEHIND,), (1,), workspace.storage_offset() + workspace.numel())
 
 
 def activation64(g, act):
@@ -63,10 +77,12 @@ def test_gated_against_float64(gpu, rows, inputs, hidden, act, pad, dtype):
     xd, dhd, wd = padded(x, pad, gpu), padded(dh, pad, gpu), w.to(gpu)
     h_store, h = guarded(rows, hidden, pad, dtype, gpu)
     dx_store, dx = guarded(rows, inputs, pad, dtype, gpu)
-    dw = torch.full((2, hidden, inputs), 7.0, dtype=dtype, device=gpu)
-    K.gated_forward(xd, wd, h, activation=act, workspace=workspace_for(x, w, gpu, False))
-    K.gated_backward(xd, wd, dhd, dx, dw, activation=act, workspace=workspace_for(x, w, gpu, True))
+    past_dw, dw = flat((2, hidden, inputs), dtype, gpu)
+    spaces = [workspace_for(x, w, gpu, backward) for backward in (False, True)]
+    K.gated_forward(xd, wd, h, activation=act, workspace=spaces[0])
+    K.gated_backward(xd, wd, dhd, dx, dw, activation=act, workspace=spaces[1])
     torch.cuda.synchronize()
+    assert (past_dw == 7).all() and all((behind(space) == 0xff).all() for space in spaces)
 
     x64, w64, dh64 = x.double(), w.double(), dh.double()
     gate, up = x64 @ w64[0].t(), x64 @ w64[1].t()
@@ -111,7 +127,7 @@ def test_gated_against_float64(gpu, rows, inputs, hidden, act, pad, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,inputs,hidden", [(1, 40, 24), (3, 7, 5), (100, 72, 130), (1000, 136, 264), (700, 123, 300),
-                                                (2100, 64, 40), (16, 512, 520)])
+                                                (2100, 64, 40), (16, 512, 520), (123, 1620, 76), (65, 1001, 1)])
 def test_small_integers_are_exact(gpu, rows, inputs, hidden, dtype):
     """Sparse values of -1, 0 and 1 with relu: every sum is a whole number that fp32 holds, dg and du at most 128, so
     the outputs are float64's rounded once.  A missing, doubled or misplaced term shows."""
@@ -133,8 +149,9 @@ def test_small_integers_are_exact(gpu, rows, inputs, hidden, dtype):
     assert torch.equal(h.cpu().double(), gate.clamp(min=0) * up)
     for dw_type in (dtype, torch.float32):
         dx = torch.empty(rows, inputs, dtype=dtype, device=gpu)
-        dw = torch.empty(2, hidden, inputs, dtype=dw_type, device=gpu)
+        past_dw, dw = flat((2, hidden, inputs), dw_type, gpu)
         K.gated_backward(xd, wd, dhd, dx, dw, activation="relu", workspace=workspace_for(xd, wd, gpu, True))
+        assert (past_dw == 7).all()
         assert torch.equal(dx.cpu(), (dg @ w[0] + du @ w[1]).to(dtype))
         assert torch.equal(dw.cpu(), torch.stack((dg.t() @ x, du.t() @ x)).to(dw_type))
 
