@@ -6,6 +6,11 @@
 // An entry whose index lies outside [0, classes) is padding; a row without entries (or whose entries are all -infinity)
 // and a row of weight 0 have loss 0 and gradient 0 whatever their logits hold.
 //
+// Bound by HBM where rows are long: 4096 x 32768 bf16 with 64 entries 118 us for loss and gradient (4.6 TB/s of logits and
+// gradient, a copy of the same bytes 98 us), the gradient alone of 1000 x 50021 fp32 94 us (4.3 TB/s); what is left are
+// the entries' scattered reads and writes (112 us with one entry).  Short rows are bound by their chain of loads and
+// reductions: 2048 x 101 fp32 6 us, under the host's 8.
+//
 // One group of threads a row, the entries in LDS.  Exponents are taken of (z - max z) / T, so that their rounding is
 // relative to the distance from the row's maximum, where the weight lies; sums are fp32 per thread and in a fixed
 // order, the few terms of the loss in 64 bits.  The gradient is written for all classes first; then, behind a barrier,

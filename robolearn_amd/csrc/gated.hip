@@ -10,7 +10,14 @@
 // dW = [dg du]^T x one product of 2 H rows; dg and du are rounded to the operands' type once, as matrix operands have
 // to be.
 //
-// fp32 operands take the three-piece bf16 products of gemm_split.hip and one pass for the gating.
+// What bounds the large sizes is the K loop: 8192 rows, 1024 inputs, 4096 hidden in bf16 take 133 us forward (1.03 PFLOP/s;
+// a library product of the same sizes alone 116 us) and 385 us backward (1.07 PFLOP/s with the recomputation), the matrix
+// cores busy 48 % of the cycles in the projections and 59 % in the gradients (the epilogues' VALU work, 19 % of the
+// cycles, overlaps nothing on tiles of 256: one workgroup a CU).  Small sizes are one chain of loads, products and
+// stores behind the launch: see stream_kernel and the plans.
+//
+// fp32 operands take the three-piece bf16 products of gemm_split.hip and one pass for the gating (2048 x 256 x 1024
+// backward 76 us: products of 19, 19 and 24 us, the pass 8 us at 5 TB/s, two sums of 5 us).
 #include "gemm.hpp"
 
 #include <algorithm>
@@ -512,7 +519,8 @@ struct Share {
 };
 
 // dx and dW side by side in one launch, the workgroups with more of K first: together they fill the CUs where each alone
-// would not (8192 x 1024 x 4096: 128 tiles of 256 x 256 each).
+// would not (8192 x 1024 x 4096: 128 tiles of 256 x 256 each; 255 us together, 2 x 148 us one after the other on tiles of
+// 128 x 128).
 template <typename T, int Edge>
 __global__ __launch_bounds__(Waves<Edge>::kThreads, 1) void gradients_kernel(Share dx, Share dw, int dw_first) {
     __shared__ __attribute__((aligned(1024))) unsigned short stage0[stage_size<Edge, Edge>()];
@@ -613,7 +621,9 @@ void launch_projection(const Product& p, int edge, hipStream_t stream) {
 // A workgroup makes 16 hidden values of up to 16 Tiles rows of x: its 4 waves take turns over K, 64 values a step, whose
 // pieces each lane loads straight into the fragments of v_mfma_f32_16x16x32 (lane l: weight row, or row of x, l % 16,
 // and K 16 (l / 16) .. + 15 of the step, so that a row's 128 bytes are read by two instructions), and the waves' sums
-// meet in LDS.  No staging: all loads of four steps are in flight at once.  Rows of any alignment.
+// meet in LDS.  No staging, and no barrier before the end; rows of any alignment.  Bound by the weights' stream: one row over
+// 2 x 4096 x 1024 bf16 5.1 us (3.3 TB/s, the launch included), over 2 x 16384 x 4096 57 us (4.7 TB/s).  64 rows x 512 x 2048
+// fp16 6.2 us, on tiles of 64 7.0 us; past 64 rows the tiles are the faster ones.
 constexpr int kStreamRows = 64;  // most rows
 
 struct __attribute__((packed, aligned(2))) Piece {

@@ -199,6 +199,8 @@ __device__ __forceinline__ int ties_below(double border, u64 above, u64 tie, int
 // ---------------------------------------------------------------------------
 // Up to 1024 classes: Lanes lanes a row (16: four rows a wave share its instructions), E consecutive classes a lane
 // ---------------------------------------------------------------------------
+// Bound by instructions: 32768 x 256 bf16 without filters 14.8 us (200 vector instructions a row, half of them the
+// weights'; 23.9 us with a wave a row), with top-p 40 us (about 15 bisection steps over all weights).
 constexpr int kShortThreads = 256;
 
 template <int Lanes>
@@ -388,6 +390,9 @@ __global__ __launch_bounds__(kShortThreads) void sample_short(Params p) {
 // ---------------------------------------------------------------------------
 // Longer rows: one workgroup a row
 // ---------------------------------------------------------------------------
+// 256 x 131072 bf16 (16 us to read at a copy's rate): greedy 21 us, top-k 64 with top-p 25 us, no filter 53 us, top-p alone 72
+// to 102 us.  Where all of a row is weighed, the weights' instructions bound it: about 24 a class, 27 us a pass of 128
+// classes a thread.  One row of 32768 fp32 with top-k and top-p: 12 us, a chain of 14 barriers.
 constexpr int kBins = 1024;
 constexpr int kBinsPerLane = kBins / kWave;
 constexpr float kBinsPerUnit = 32.0f;  // linear bins of 1/32 of (max - z) / T: 32 units until the last one
