@@ -260,7 +260,9 @@ void launch_teams(const Params& p, hipStream_t stream) {
 
 // The smallest team whose registers hold the row, 8 chunks a thread where that reaches: 4096 x 32768 bf16, loss and
 // gradient, 121 us on 512 threads of 8 chunks, 131 on 256 of 16, 139 on 1024 of 4, 174 reading memory twice (a copy of the
-// same bytes: 98 us).
+// same bytes: 98 us).  Twice that: 2048 x 65536 131 us on 512 threads of 16 chunks, 169 on 1024 of 8, the gradient alone 130
+// against 116.  Streaming such rows would be faster for the loss alone, which reads a row once either way (48 us against
+// 62), but the loss would then differ in its last bits from the one that comes with the gradient.
 template <typename T, bool Backward>
 void launch(const Params& p, hipStream_t stream) {
     const int chunks = static_cast<int>(ceil_div(p.classes, T::kPerChunk));
@@ -274,7 +276,8 @@ void launch(const Params& p, hipStream_t stream) {
     else if (chunks <= 256 * 4) launch_teams<T, 256, 4, Backward>(p, stream);
     else if (chunks <= 256 * 8) launch_teams<T, 256, 8, Backward>(p, stream);
     else if (chunks <= 512 * 8) launch_teams<T, 512, 8, Backward>(p, stream);
-    else if (chunks <= 1024 * 8) launch_teams<T, 1024, 8, Backward>(p, stream);
+    else if (!Backward && chunks <= 512 * 16) launch_teams<T, 512, 16, false>(p, stream);
+    else if (Backward && chunks <= 1024 * 8) launch_teams<T, 1024, 8, true>(p, stream);
     else if (chunks <= 1024 * 16) launch_teams<T, 1024, 16, Backward>(p, stream);
     else launch_teams<T, 1024, 0, Backward>(p, stream);
 }
