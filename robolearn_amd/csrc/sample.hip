@@ -209,8 +209,9 @@ __device__ __forceinline__ int ties_below(double border, u64 above, u64 tie, int
 // ---------------------------------------------------------------------------
 // Up to 1024 classes: Lanes lanes a row (16: four rows a wave share its instructions), E consecutive classes a lane
 // ---------------------------------------------------------------------------
-// Bound by instructions: 32768 x 256 bf16 without filters 12.9 us (23.9 with a wave a row), most of them the
-// weights'; the chosen class is found in whole numbers (14.8 us with a comparison in 64 bits at each class), with top-p 40 us (about 15 bisection steps over all weights).
+// Bound by instructions, most of them the weights': 32768 x 256 bf16 without filters 12.9 us (23.9 with a wave a row; 14.8
+// with comparisons in doubles, not whole numbers, to find the chosen class), greedy 9.0 us, with top-p 40 us (about 15
+// bisection steps over all weights).
 constexpr int kShortThreads = 256;
 
 template <int Lanes>
@@ -298,10 +299,18 @@ __global__ __launch_bounds__(kShortThreads) void sample_short(Params p) {
         if (lane == 0) nothing_drawn(p, r, s.valid);
         return;
     }
+    if (s.one()) {
+        unsigned back = 0;  // the first class of the maximum, counted from the end
+#pragma unroll
+        for (int e = 0; e < E; ++e) back = max(back, z[e] == m ? ~static_cast<unsigned>(first + e) : 0u);
+        back = L::max(back);
+        if (lane == 0) drawn(p, r, ~back, m, m, s.per_t, 1ULL << 43);
+        return;
+    }
     const Weights weight(table, m, s.per_t);
     u64 w[E];
     weight(z, w);
-    if (s.one() || (s.top_k > 0 && s.top_k < p.classes) || s.top_p < 1.0) {
+    if ((s.top_k > 0 && s.top_k < p.classes) || s.top_p < 1.0) {
         unsigned key[E];  // 0: masked
         const unsigned high = (ordered(m) >> kShift) + 1;
         unsigned far = 0;
@@ -311,8 +320,9 @@ __global__ __launch_bounds__(kShortThreads) void sample_short(Params p) {
             if (key[e]) far = max(far, high - key[e]);
         }
         const unsigned low = high - L::max(far);
+        // (inlined by force: left as a call, one of these puts the row into scratch memory, 12.9 -> 18.3 us)
         // the largest key at which `reached` holds, which it does at `floor`; all keys lie in [low, high]
-        const auto bisect = [&](unsigned floor, auto reached) {
+        const auto bisect = [&](unsigned floor, auto reached) __attribute__((always_inline)) {
             if (floor == high) return high;
             int bit = 31 - __clz(floor ^ high);
             unsigned border = high >> bit >> 1 << bit << 1;
@@ -320,20 +330,20 @@ __global__ __launch_bounds__(kShortThreads) void sample_short(Params p) {
                 if (reached(border | (1u << bit))) border |= 1u << bit;
             return border;
         };
-        const auto count_from = [&](unsigned k) {
+        const auto count_from = [&](unsigned k) __attribute__((always_inline)) {
             int n = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) n += key[e] >= k;
             return L::total(n);
         };
-        const auto mass_from = [&](unsigned k) {
+        const auto mass_from = [&](unsigned k) __attribute__((always_inline)) {
             u64 sum = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) sum += key[e] >= k ? w[e] : 0;
             return L::total(sum);
         };
         // what a token of key k weighs (the key occurs)
-        const auto weight_at = [&](unsigned k) {
+        const auto weight_at = [&](unsigned k) __attribute__((always_inline)) {
             unsigned lo = 0, hi = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
@@ -344,25 +354,20 @@ __global__ __launch_bounds__(kShortThreads) void sample_short(Params p) {
         };
         unsigned border = 1;  // keys above it stay, and the first `ties` of those equal to it
         int ties = INT_MAX;
-        if (s.one()) {
-            border = high;
-            ties = 1;
-        } else {
-            if (s.top_k > 0 && s.top_k < count_from(1)) {
-                border = bisect(low, [&](unsigned k) { return count_from(k) >= s.top_k; });
-                ties = s.top_k - count_from(border + 1);
-            }
-            if (s.top_p < 1.0) {
-                const bool limited = ties != INT_MAX;
-                const u64 tie = limited ? weight_at(border) : 0;
-                const u64 above = mass_from(limited ? border + 1 : 1);
-                const double mass = s.top_p * static_cast<double>(above + (limited ? tie * static_cast<u64>(ties) : 0));
-                if (static_cast<double>(above) >= mass) {
-                    border = bisect(max(border, low), [&](unsigned k) { return static_cast<double>(mass_from(k)) >= mass; });
-                    ties = ties_below(mass, mass_from(border + 1), weight_at(border), p.classes);
-                } else if (tie > 0) {
-                    ties = ties_below(mass, above, tie, ties);
-                }
+        if (s.top_k > 0 && s.top_k < count_from(1)) {
+            border = bisect(low, [&](unsigned k) { return count_from(k) >= s.top_k; });
+            ties = s.top_k - count_from(border + 1);
+        }
+        if (s.top_p < 1.0) {
+            const bool limited = ties != INT_MAX;
+            const u64 tie = limited ? weight_at(border) : 0;
+            const u64 above = mass_from(limited ? border + 1 : 1);
+            const double mass = s.top_p * static_cast<double>(above + (limited ? tie * static_cast<u64>(ties) : 0));
+            if (static_cast<double>(above) >= mass) {
+                border = bisect(max(border, low), [&](unsigned k) { return static_cast<double>(mass_from(k)) >= mass; });
+                ties = ties_below(mass, mass_from(border + 1), weight_at(border), p.classes);
+            } else if (tie > 0) {
+                ties = ties_below(mass, above, tie, ties);
             }
         }
         int equal = 0;
