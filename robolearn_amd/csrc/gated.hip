@@ -281,11 +281,12 @@ constexpr int stage_size() {
     return (TM + TN) * kDepth;
 }
 
-// Tile `block` of the product's `blocks` by a workgroup of WavesM x WavesN waves.  stage0, stage1: two LDS objects of
-// stage_size (the compiler then tells reads of one from the DMA into the other).
-template <typename T, bool AMN, bool BMN, int TM, int TN, int WavesM, int WavesN, int Out, int Kind>
-__device__ __forceinline__ void make_tile(const Product& p, int tiles_m, int tiles_n, int block, int blocks,
-                                          unsigned short* stage0, unsigned short* stage1) {
+// Tile `block` of the product's `blocks` by a workgroup of WavesM x WavesN waves; Again: then the tiles `stride` further
+// on, of which the first K tile arrives under the epilogue (K must be an even number of K tiles where there are any).
+// stage0, stage1: two LDS objects of stage_size (the compiler then tells reads of one from the DMA into the other).
+template <typename T, bool AMN, bool BMN, int TM, int TN, int WavesM, int WavesN, int Out, int Kind, bool Again>
+__device__ __forceinline__ void make_tiles(const Product& p, int tiles_m, int tiles_n, int block, int blocks, int stride,
+                                           unsigned short* stage0, unsigned short* stage1) {
     constexpr int kWaves = WavesM * WavesN;
     constexpr int kThreadCount = kWaves * kWave;
     constexpr int MI = TM / WavesM / 32, NJ = TN / WavesN / 32;
@@ -298,8 +299,8 @@ __device__ __forceinline__ void make_tile(const Product& p, int tiles_m, int til
     const int wm = wave / WavesN, wn = wave % WavesN;
     int tm, tn, split;
     tile_of(block, blocks, tiles_m, tiles_n, tm, tn, split);
-    const int m0 = tm * TM, n0 = tn * kOutN;
-    const int rows_a = min(TM, p.m - m0), rows_b = min(kOutN, p.n - n0);
+    int m0 = tm * TM, n0 = tn * kOutN;
+    bool more = Again && block + stride < blocks;
 
     Loader<AMN, TM, kWaves> la;
     Loader<BMN, TN, kWaves> lb;
@@ -310,26 +311,28 @@ __device__ __forceinline__ void make_tile(const Product& p, int tiles_m, int til
     const int first_tile = split * p.tiles_per_split;
     const int last_tile = min(first_tile + p.tiles_per_split, per_segment * p.segments);
     int segment = first_tile / per_segment, k0 = (first_tile % per_segment) * kDepth;
+    int next_m = m0, next_n = n0;  // the tile that is fetched
     const auto fetch = [&](unsigned short* stage) {
         const int depth = min(kDepth, p.k - k0);
-        const unsigned short* a = p.a + segment * p.seg_a + (AMN ? k0 * p.lda + m0 : m0 * p.lda + k0);
-        const unsigned short* b = p.b + segment * p.seg_b + (BMN ? k0 * p.ldb + n0 : n0 * p.ldb + k0);
+        const int rows_a = min(TM, p.m - next_m), rows_b = min(kOutN, p.n - next_n);
+        const unsigned short* a = p.a + segment * p.seg_a + (AMN ? k0 * p.lda + next_m : next_m * p.lda + k0);
+        const unsigned short* b = p.b + segment * p.seg_b + (BMN ? k0 * p.ldb + next_n : next_n * p.ldb + k0);
         // M/N-contiguous rows may be read up to their next multiple of 8, which the pitch covers
         la.fetch(a, nullptr, p.lda, AMN ? (rows_a + 7) / 8 * 8 : rows_a, depth, stage, wave);
         lb.fetch(b, kGated ? b + p.up : nullptr, p.ldb, BMN ? (rows_b + 7) / 8 * 8 : rows_b, depth,
                  stage + TM * kDepth, wave);
         k0 += kDepth;
-        if (k0 >= p.k) k0 = 0, ++segment;
+        if (k0 < p.k) return;
+        k0 = 0;
+        if constexpr (!Again) {
+            ++segment;
+        } else if (more) {
+            tile_of(block + stride, blocks, tiles_m, tiles_n, tm, tn, split);
+            next_m = tm * TM, next_n = tn * kOutN;
+        }
     };
 
     gemm::f32x16_t acc[MI][NJ];
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
-
     Reader<T, AMN, TM, MI> ra;
     Reader<T, BMN, TN, NJ> rb;
     ra.init(wm * (TM / WavesM), lane);
@@ -359,141 +362,156 @@ __device__ __forceinline__ void make_tile(const Product& p, int tiles_m, int til
 #pragma unroll
         for (int s = 0; s + 1 < kSteps; ++s) {
             read(stage, s + 1, (s + 1) % 2);
-            if (s == 0 && late && kt >= 1 && kt + 1 < tiles) fetch(const_cast<unsigned short*>(other));
+            if (s == 0 && late && kt >= 1 && (more || kt + 1 < tiles)) fetch(const_cast<unsigned short*>(other));
             multiply(s % 2);
         }
         if (kt + 1 < tiles) {
             stage_barrier();
-            if (!late && kt + 2 < tiles) fetch(stage);
+            if (!late && (more || kt + 2 < tiles)) fetch(stage);
             read(other, 0, 0);
         }
         multiply((kSteps - 1) % 2);
     };
     fetch(stage0);
     stage_barrier();
-    if (tiles > 1) fetch(stage1);
-    read(stage0, 0, 0);
-    int kt = 0;
-    for (; kt + 1 < tiles; kt += 2) {
-        k_tile(kt, stage0, stage1);
-        k_tile(kt + 1, stage1, stage0);
-    }
-    if (kt < tiles) k_tile(kt, stage0, stage1);
-
-    // accumulator element v of lane l: column l % 32, row 8 (v / 4) + 4 (l / 32) + v % 4 of its 32 x 32 block
-    const int col = lane % 32, row4 = 4 * (lane / 32);
-    if constexpr (!kGated) {
-        if (p.d32) {
-            const bool direct = p.splits == 1;
-            float* d = p.d32 + (direct ? 0 : static_cast<long long>(split) * p.m * p.n);
-            const long long ldd = direct ? p.ldd : p.n;
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    const int c = n0 + wn * (TN / WavesN) + 32 * j + col;
-                    if (c >= p.n) continue;
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) {
-                        const int r = m0 + wm * (TM / WavesM) + 32 * i + 8 * (v / 4) + row4 + v % 4;
-                        const long long to = direct ? folded(r, p.fold, p.fold_to) : r;
-                        if (r < p.m && to >= 0) d[to * ldd + c] = acc[i][j][v];
-                    }
-                }
-            return;
-        }
-    }
-
-    // 16-bit outputs leave through LDS, whole tile rows at a time: in MI passes of 32 rows from each row of waves
-    constexpr int kPitch = kOutN + 8;
-    constexpr int kPassRows = 32 * WavesM;
-    static_assert(kPassRows * kPitch <= kStage, "a pass fits a stage");
-    constexpr int kChunks = kOutN / 8;  // 16-byte pieces of a tile row
-    // rows of `out`, whose first `columns` values exist, from LDS
-    const auto leave = [&](const unsigned short* lds, unsigned short* out, long long ld, int columns, int pass) {
-        const bool wide = reinterpret_cast<std::uintptr_t>(out) % 16 == 0 && ld % 8 == 0;
-        for (int q = static_cast<int>(threadIdx.x); q < kPassRows * kChunks; q += kThreadCount) {
-            const int local = q / kChunks, c = n0 + q % kChunks * 8;
-            const int r = m0 + local / 32 * (TM / WavesM) + 32 * pass + local % 32;
-            const long long row = kGated ? r : folded(r, p.fold, p.fold_to);
-            if (r >= p.m || row < 0 || c >= columns) continue;
-            const unsigned short* in = lds + local * kPitch + q % kChunks * 8;
-            unsigned short* to = out + row * ld + c;
-            if (wide && c + 8 <= columns) {
-                *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(in);
-            } else {
-                for (int e = 0; e < 8 && c + e < columns; ++e) to[e] = in[e];
-            }
-        }
-    };
-    // backward: this thread's pieces of dh, all of them before the first pass waits for one
-    constexpr int kPieces = (kPassRows * kChunks + kThreadCount - 1) / kThreadCount;
-    static_assert(kPassRows * kChunks % kThreadCount == 0, "whole pieces");
-    u32x4 dh_pieces[Out == kBackward ? MI : 1][kPieces];
-    if constexpr (Out == kBackward) {
-        const bool wide = reinterpret_cast<std::uintptr_t>(p.dh) % 16 == 0 && p.ld_dh % 8 == 0;
+    for (;;) {
+        if (tiles > 1) fetch(stage1);
+        read(stage0, 0, 0);
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int k = 0; k < kPieces; ++k) {
-                const int q = static_cast<int>(threadIdx.x) + k * kThreadCount;
-                const int local = q / kChunks, c = n0 + q % kChunks * 8;
-                const int r = m0 + local / 32 * (TM / WavesM) + 32 * i + local % 32;
-                u32x4 piece{0u, 0u, 0u, 0u};
-                if (r < p.m && c < p.n) {
-                    const unsigned short* from = p.dh + r * p.ld_dh + c;
-                    if (wide && c + 8 <= p.n) {
-                        piece = *reinterpret_cast<const u32x4*>(from);
-                    } else {
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            if (c + e < p.n) piece[e / 2] |= static_cast<unsigned>(from[e]) << (16 * (e % 2));
+                for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+        int kt = 0;
+        for (; kt + 1 < tiles; kt += 2) {
+            k_tile(kt, stage0, stage1);
+            k_tile(kt + 1, stage1, stage0);
+        }
+        if (kt < tiles) k_tile(kt, stage0, stage1);
+
+        // accumulator element v of lane l: column l % 32, row 8 (v / 4) + 4 (l / 32) + v % 4 of its 32 x 32 block
+        const int col = lane % 32, row4 = 4 * (lane / 32);
+        if constexpr (!kGated) {
+            if (p.d32) {
+                const bool direct = p.splits == 1;
+                float* d = p.d32 + (direct ? 0 : static_cast<long long>(split) * p.m * p.n);
+                const long long ldd = direct ? p.ldd : p.n;
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        const int c = n0 + wn * (TN / WavesN) + 32 * j + col;
+                        if (c >= p.n) continue;
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) {
+                            const int r = m0 + wm * (TM / WavesM) + 32 * i + 8 * (v / 4) + row4 + v % 4;
+                            const long long to = direct ? folded(r, p.fold, p.fold_to) : r;
+                            if (r < p.m && to >= 0) d[to * ldd + c] = acc[i][j][v];
+                        }
+                    }
+                return;
+            }
+        }
+
+        // 16-bit outputs leave through LDS, whole tile rows at a time: in MI passes of 32 rows from each row of waves
+        constexpr int kPitch = kOutN + 8;
+        constexpr int kPassRows = 32 * WavesM;
+        static_assert((Out == kBackward ? 2 : 1) * kPassRows * kPitch <= kStage, "a pass fits a stage");
+        constexpr int kChunks = kOutN / 8;  // 16-byte pieces of a tile row
+        // rows of `out`, whose first `columns` values exist, from LDS
+        const auto leave = [&](const unsigned short* lds, unsigned short* out, long long ld, int columns, int pass) {
+            const bool wide = reinterpret_cast<std::uintptr_t>(out) % 16 == 0 && ld % 8 == 0;
+            for (int q = static_cast<int>(threadIdx.x); q < kPassRows * kChunks; q += kThreadCount) {
+                const int local = q / kChunks, c = n0 + q % kChunks * 8;
+                const int r = m0 + local / 32 * (TM / WavesM) + 32 * pass + local % 32;
+                const long long row = kGated ? r : folded(r, p.fold, p.fold_to);
+                if (r >= p.m || row < 0 || c >= columns) continue;
+                const unsigned short* in = lds + local * kPitch + q % kChunks * 8;
+                unsigned short* to = out + row * ld + c;
+                if (wide && c + 8 <= columns) {
+                    *reinterpret_cast<u32x4*>(to) = *reinterpret_cast<const u32x4*>(in);
+                } else {
+                    for (int e = 0; e < 8 && c + e < columns; ++e) to[e] = in[e];
+                }
+            }
+        };
+        // backward: this thread's pieces of dh, all of them before the first pass waits for one
+        constexpr int kPieces = (kPassRows * kChunks + kThreadCount - 1) / kThreadCount;
+        static_assert(kPassRows * kChunks % kThreadCount == 0, "whole pieces");
+        u32x4 dh_pieces[Out == kBackward ? MI : 1][kPieces];
+        if constexpr (Out == kBackward) {
+            const bool wide = reinterpret_cast<std::uintptr_t>(p.dh) % 16 == 0 && p.ld_dh % 8 == 0;
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) {
+                    const int q = static_cast<int>(threadIdx.x) + k * kThreadCount;
+                    const int local = q / kChunks, c = n0 + q % kChunks * 8;
+                    const int r = m0 + local / 32 * (TM / WavesM) + 32 * i + local % 32;
+                    u32x4 piece{0u, 0u, 0u, 0u};
+                    if (r < p.m && c < p.n) {
+                        const unsigned short* from = p.dh + r * p.ld_dh + c;
+                        if (wide && c + 8 <= p.n) {
+                            piece = *reinterpret_cast<const u32x4*>(from);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (c + e < p.n) piece[e / 2] |= static_cast<unsigned>(from[e]) << (16 * (e % 2));
+                        }
+                    }
+                    dh_pieces[i][k] = piece;
+                }
+        }
+        unsigned short *one = stage1, *two = stage1 + kPassRows * kPitch;  // stage0 may be taking the next tile
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            lds_barrier();  // the stage is free, and the pass before has left
+            if constexpr (Out == kBackward) {
+#pragma unroll
+                for (int k = 0; k < kPieces; ++k) {
+                    const int q = static_cast<int>(threadIdx.x) + k * kThreadCount;
+                    *reinterpret_cast<u32x4*>(one + q / kChunks * kPitch + q % kChunks * 8) = dh_pieces[i][k];
+                }
+                lds_barrier();
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                unsigned short* lds_one = one + (wm * 32 + 8 * (v / 4) + row4 + v % 4) * kPitch + col;
+                if constexpr (!kGated) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) lds_one[wn * (TN / WavesN) + 32 * j] = T::rounded(acc[i][j][v]);
+                } else {
+                    lds_one += wn * 32;
+                    const float up = acc[i][1][v];
+                    float value, slope;
+                    activate<Kind>(acc[i][0][v], value, slope);
+                    if constexpr (Out == kForward) {
+                        *lds_one = T::rounded(value * up);
+                    } else {
+                        const float dh = T::value(*lds_one);  // 0 past the last column, and so is what leaves for it
+                        *lds_one = T::rounded(dh * up * slope);
+                        two[lds_one - one] = T::rounded(dh * value);
                     }
                 }
-                dh_pieces[i][k] = piece;
             }
-    }
-    unsigned short *one = stage0, *two = stage1;
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        lds_barrier();  // the stages are free, and the pass before has left
-        if constexpr (Out == kBackward) {
-#pragma unroll
-            for (int k = 0; k < kPieces; ++k) {
-                const int q = static_cast<int>(threadIdx.x) + k * kThreadCount;
-                *reinterpret_cast<u32x4*>(one + q / kChunks * kPitch + q % kChunks * 8) = dh_pieces[i][k];
-            }
-            lds_barrier();
-        }
-#pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            unsigned short* lds_one = one + (wm * 32 + 8 * (v / 4) + row4 + v % 4) * kPitch + col;
-            if constexpr (!kGated) {
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) lds_one[wn * (TN / WavesN) + 32 * j] = T::rounded(acc[i][j][v]);
+            // the first K tile of the next one has landed: the barrier before the first store, which would be waited for too
+            if (Again && i == 0) stage_barrier();
+            else lds_barrier();
+            if constexpr (Out == kPlain) {
+                leave(one, p.d, p.ldd, p.n, i);
+            } else if constexpr (Out == kForward) {
+                leave(one, p.h, p.ld_h, p.n, i);
             } else {
-                lds_one += wn * 32;
-                const float up = acc[i][1][v];
-                float value, slope;
-                activate<Kind>(acc[i][0][v], value, slope);
-                if constexpr (Out == kForward) {
-                    *lds_one = T::rounded(value * up);
-                } else {
-                    const float dh = T::value(*lds_one);  // 0 past the last column, and so is what leaves for it
-                    *lds_one = T::rounded(dh * up * slope);
-                    two[lds_one - one] = T::rounded(dh * value);
-                }
+                leave(one, p.dpre, 2 * p.pitch, static_cast<int>(p.pitch), i);
+                leave(two, p.dpre + p.pitch, 2 * p.pitch, static_cast<int>(p.pitch), i);
             }
         }
-        lds_barrier();
-        if constexpr (Out == kPlain) {
-            leave(one, p.d, p.ldd, p.n, i);
-        } else if constexpr (Out == kForward) {
-            leave(one, p.h, p.ld_h, p.n, i);
-        } else {
-            leave(one, p.dpre, 2 * p.pitch, static_cast<int>(p.pitch), i);
-            leave(two, p.dpre + p.pitch, 2 * p.pitch, static_cast<int>(p.pitch), i);
-        }
+        if (!more) return;
+        lds_barrier();  // stage1 is free
+        block += stride;
+        m0 = next_m, n0 = next_n;
+        more = block + stride < blocks;
     }
 }
 
@@ -504,12 +522,19 @@ struct Waves {
     static constexpr int kThreads = kM * kN * kWave;
 };
 
+// Whether a workgroup goes on to other tiles: 8192 x 512 -> 2048 43 -> 40.5 us, 16384 x 2048 -> 8192 910 -> 887 us; the
+// backward projection, whose epilogue waits for its own loads, gains nothing.
+template <int Edge, int Out>
+__host__ __device__ constexpr bool tiles_follow() {
+    return Edge == 256 && Out == kForward;
+}
+
 template <typename T, int Edge, int Out, int Kind>
 __global__ __launch_bounds__(Waves<Edge>::kThreads, 1) void project_kernel(Product p, int tiles_m, int tiles_n) {
     __shared__ __attribute__((aligned(1024))) unsigned short stage0[stage_size<Edge, Edge>()];
     __shared__ __attribute__((aligned(1024))) unsigned short stage1[stage_size<Edge, Edge>()];
-    make_tile<T, false, false, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, Out, Kind>(
-        p, tiles_m, tiles_n, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x), stage0, stage1);
+    make_tiles<T, false, false, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, Out, Kind, tiles_follow<Edge, Out>()>(
+        p, tiles_m, tiles_n, static_cast<int>(blockIdx.x), tiles_m * tiles_n, static_cast<int>(gridDim.x), stage0, stage1);
 }
 
 // One of the two gradient products: its tiles, and its workgroups (0: not asked for).
@@ -527,11 +552,11 @@ __global__ __launch_bounds__(Waves<Edge>::kThreads, 1) void gradients_kernel(Sha
     __shared__ __attribute__((aligned(1024))) unsigned short stage1[stage_size<Edge, Edge>()];
     const int block = static_cast<int>(blockIdx.x);
     if (dw_first ? block >= dw.blocks : block < dx.blocks)
-        make_tile<T, false, true, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, kPlain, kRelu>(
-            dx.p, dx.tiles_m, dx.tiles_n, dw_first ? block - dw.blocks : block, dx.blocks, stage0, stage1);
+        make_tiles<T, false, true, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, kPlain, kRelu, false>(
+            dx.p, dx.tiles_m, dx.tiles_n, dw_first ? block - dw.blocks : block, dx.blocks, 0, stage0, stage1);
     else
-        make_tile<T, true, true, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, kPlain, kRelu>(
-            dw.p, dw.tiles_m, dw.tiles_n, dw_first ? block : block - dx.blocks, dw.blocks, stage0, stage1);
+        make_tiles<T, true, true, Edge, Edge, Waves<Edge>::kM, Waves<Edge>::kN, kPlain, kRelu, false>(
+            dw.p, dw.tiles_m, dw.tiles_n, dw_first ? block : block - dx.blocks, dw.blocks, 0, stage0, stage1);
 }
 
 // What a tile takes: up to `beside` workgroups a CU, r of them on each; us per 64 of K and us beside that.  Measured with
@@ -603,7 +628,10 @@ GradientPlan gradient_plan(long long dx_m, long long dw_m, long long n, long lon
 template <typename T, int Edge, int Out, int Kind>
 void launch_projection(const Product& p, hipStream_t stream) {
     const long long tiles_m = ceil_div(p.m, Edge), tiles_n = ceil_div(p.n, Edge / 2);
-    hipLaunchKernelGGL((project_kernel<T, Edge, Out, Kind>), dim3(static_cast<unsigned>(tiles_m * tiles_n)),
+    // an even number of K tiles: each CU's workgroup takes its tiles one after the other
+    const bool again = tiles_follow<Edge, Out>() && ceil_div(p.k, kDepth) % 2 == 0;
+    const long long groups = again ? std::min<long long>(tiles_m * tiles_n, kCus) : tiles_m * tiles_n;
+    hipLaunchKernelGGL((project_kernel<T, Edge, Out, Kind>), dim3(static_cast<unsigned>(groups)),
                        dim3(Waves<Edge>::kThreads), 0, stream, p, static_cast<int>(tiles_m), static_cast<int>(tiles_n));
     check_launch("Launch gated projection");
 }

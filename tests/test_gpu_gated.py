@@ -125,6 +125,13 @@ def test_gated_against_float64(gpu, rows, inputs, hidden, act, pad, dtype):
         assert ((dw[half_w].cpu().double() - exact).abs() <= product_bound(d.t(), e.t(), x64, exact)).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("inputs,act,pad", [(100, "gelu", 0), (150, "silu", 3), (520, "relu", 8), (1000, "silu", 0)])
+def test_two_tiles_a_workgroup(gpu, inputs, act, pad, dtype):
+    """512 tiles of 256 x 256 on 256 CUs, ragged at both ends, over 2, 3, 9 and 16 K tiles."""
+    test_gated_against_float64(gpu, 8155, inputs, 2043, act, pad, dtype)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,inputs,hidden", [(1, 40, 24), (3, 7, 5), (100, 72, 130), (1000, 136, 264), (700, 123, 300),
                                                 (2100, 64, 40), (16, 512, 520), (123, 1620, 76), (65, 1001, 1)])
