@@ -10,10 +10,10 @@
 // dW = [dg du]^T x one product of 2 H rows; dg and du are rounded to the operands' type once, as matrix operands have
 // to be.
 //
-// What bounds the large sizes is the K loop: 8192 rows, 1024 inputs, 4096 hidden in bf16 take 133 us forward (1.03 PFLOP/s;
+// What bounds the large sizes is the K loop: 8192 rows, 1024 inputs, 4096 hidden in bf16 take 127 us forward (1.08 PFLOP/s;
 // a library product of the same sizes alone 116 us) and 385 us backward (1.07 PFLOP/s with the recomputation), the matrix
-// cores busy 48 % of the cycles in the projections and 59 % in the gradients (the epilogues' VALU work, 19 % of the
-// cycles, overlaps nothing on tiles of 256: one workgroup a CU).  Small sizes are one chain of loads, products and
+// cores busy 51 % of the cycles in the forward projection and 59 % in the gradients (the epilogues' VALU work, about a
+// fifth of the cycles, overlaps only loads on tiles of 256: one workgroup a CU).  Small sizes are one chain of loads, products and
 // stores behind the launch: see stream_kernel and the plans.
 //
 // fp32 operands take the three-piece bf16 products of gemm_split.hip and one pass for the gating (2048 x 256 x 1024
