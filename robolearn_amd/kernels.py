@@ -485,10 +485,10 @@ def _gated_operands(x, w, activation):
 
 
 def gated_forward(x, w, h, *, activation="silu", workspace=None):
-    """h = act(x w[0]^T) * (x w[1]^T) in one launch (fp32: a product and a pass; 16-bit rows that are no multiples of 16
-    bytes are copied first past 64 rows): x [rows, inputs], w [2, hidden, inputs], h [rows, hidden], one type; x and h may
-    have row pitches.  workspace: gated_workspace bytes; calls that
-    may overlap (other streams, other graphs) need one each."""
+    """h = act(x w[0]^T) * (x w[1]^T) in one launch (fp32: a product, its sum where K is split, and a pass; 16-bit rows that
+    are no multiples of 16 bytes are copied first past 64 rows): x [rows, inputs], w [2, hidden, inputs], h [rows, hidden],
+    one type; x and h may have row pitches.  workspace: gated_workspace bytes; calls that may overlap (other streams, other
+    graphs) need one each."""
     code, rows, inputs, hidden, ldx = _gated_operands(x, w, activation)
     ld_h = _matrix(h, (rows, hidden), "h", x.dtype)
     on = _current(x, w, h, workspace)
